@@ -132,6 +132,105 @@ int ork_b200_rows_qk_rope_async(ork_npu *ctx, const float *q, const float *k, co
                                 float *Kc, float *Vc, int hstride);
 int ork_b200_argmax_scaled_async(ork_npu *ctx, const int32_t *C, const float *bs, int n, long long *idx);
 
+/* ---- Long contexts: prompt attention, a 4-bit key/value cache, attention over it, eviction -----------------------
+ * No counterpart in ork-driver, whose attention is the decode layer's over one fp32 cache. All calls take device
+ * pointers, enqueue on the context's stream and return 0, or -1 with a message and nothing queued. What only the
+ * device can see (a length or slot outside its cache) skips that sequence or row and is reported by the next
+ * ork_b200_sync. `type` is one of the three below; strides are in elements. Head size dk is 64 or 128; query head
+ * h reads kv head h / (H / Hkv), so H is a multiple of Hkv. */
+#define ORK_B200_F32 0
+#define ORK_B200_F16 1
+#define ORK_B200_BF16 2
+
+/* Attention of rows over keys: a sequence's q_start[s+1] - q_start[s] query rows are the last ones of its
+ * k_start[s+1] - k_start[s] keys (a prompt after a cached prefix; equal counts: the prompt alone). Query i of tq at
+ * position p = tk - tq + i sees key j when j <= p and (window == 0 or j > p - window or j < sinks): a sliding window
+ * of the last `window` keys, the first `sinks` keys staying visible. out = sum over the visible keys of
+ * softmax(scale * q . k) v; a row that sees no key (p < 0) gives zeros. Rows of all sequences are packed; row r of
+ * head h lies at q + r * q_ts + h * q_hs, its dk values contiguous, likewise k, v and out.
+ * type ORK_B200_F16 or ORK_B200_BF16 (inputs and output); the scores and the output are summed in fp32 and the
+ * softmax weights enter the second product rounded to `type`. Bases are 16-byte aligned, strides multiples of 8.
+ * out overlaps no input. q_start, k_start: device int [nseq + 1]; q_rows / k_rows: rows that q and out / k and v
+ * hold; max_q / max_k: the most rows of any one sequence (they size the launch). */
+typedef struct ork_b200_attn {
+  const void *q, *k, *v;
+  void *out;
+  int type, nseq, H, Hkv, dk;
+  long long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
+  const int *q_start, *k_start;
+  int q_rows, k_rows, max_q, max_k;
+  float scale;
+  int window, sinks;
+} ork_b200_attn;
+int ork_b200_attn_async(ork_npu *ctx, const ork_b200_attn *a);
+
+/* A key/value cache held in 4 bits, in the caller's device memory: codes k, v [nseq][Hkv][cap][dk/2] bytes (low
+ * nibble: the even dim) and parameters kp, vp [nseq][Hkv][cap][dk/64][2] fp16: the step and the lowest value of each
+ * 64 consecutive dims; a value is code * step + lowest. 4.5 bits a value: 144 bytes a token and kv head at dk = 128.
+ * cap is a multiple of 64; the four arrays are 16-byte aligned. */
+typedef struct ork_b200_kv4 {
+  uint8_t *k, *v;
+  ork_f16 *kp, *vp;
+  int nseq, Hkv, dk, cap;
+} ork_b200_kv4;
+
+/* Rows into the cache and back. Row t of sequence s goes to slot pos[s] + t (pos NULL: 0). The rows are packed:
+ * sequence s has rows start[s] .. start[s+1] - 1 (device int [nseq + 1]) and `rows` is the most of any sequence, or,
+ * with start NULL, `rows` each. Row r of kv head h lies at k + r * ts + h * hs (v likewise), dk contiguous values of
+ * `type`: ts = Hkv*dk, hs = dk are packed projections; ts = dk, hs = hstride*dk the decode layer's fp32 caches.
+ * The store, per 64 dims with lowest lo and largest hi, in fp32: step = f16(min((hi - lo) * (1/15), 65504)),
+ * lowest = f16(lo) saturated, code = clamp(rint((x - lowest) / step), 0, 15), 0 where the step is 0. Dims that hold
+ * a NaN or an infinity give a NaN step and lowest value: the token reads back as NaN wherever it is visible.
+ * A slot outside [0, cap) is not written (read) and reported. */
+int ork_b200_kv4_store_async(ork_npu *ctx, const ork_b200_kv4 *c, const void *k, const void *v, int type, int rows,
+                             long long ts, long long hs, const int *start, const int *pos);
+int ork_b200_kv4_load_async(ork_npu *ctx, const ork_b200_kv4 *c, void *k, void *v, int type, int rows, long long ts,
+                            long long hs, const int *start, const int *pos);
+
+/* Attention of the last T tokens of every sequence over the cache (1: a decode step; more: drafted tokens, a short
+ * prompt's rows). Sequence s holds len[s] tokens (device int [nseq], at most max_len, the new ones among them; 0
+ * leaves its rows zero); token t of T is at position len[s] - T + t and sees keys as in ork_b200_attn. q row (s, t)
+ * of head h lies at q + (s*T + t) * q_ts + h * q_hs; out is [nseq][T][H][dk]. q and out have `type`, any of the
+ * three, and are aligned to it; arithmetic is fp32-like throughout (operands of the matrix instructions are split
+ * in two halves). After an eviction positions count the kept tokens.
+ * wsum (NULL: none) [nseq][Hkv][cap] fp32: every visible key's softmax weights, summed over the T tokens and the
+ * H / Hkv heads of its kv head, are added to its entry. The first call with a larger problem grows the context's
+ * workspace (make one before capturing a CUDA graph); calls on one context run one after another. */
+typedef struct ork_b200_kv4_attn {
+  const void *q;
+  void *out;
+  int type, H, T;
+  long long q_ts, q_hs;
+  const int *len;
+  int max_len;
+  float scale;
+  int window, sinks;
+  float *wsum;
+} ork_b200_kv4_attn;
+int ork_b200_kv4_attn_async(ork_npu *ctx, const ork_b200_kv4 *c, const ork_b200_kv4_attn *a);
+
+/* Eviction from a cache by accumulated attention weight. Of the n = len[s] tokens of each sequence and kv head,
+ * min(n, keep) are kept: the first `sinks`, the last `recent`, then those with the largest score [nseq][Hkv][cap]
+ * (ties: the lowest slot; a NaN counts as minus infinity); sinks + recent <= keep. The kept rows move, in their
+ * order, from each of `nplanes` source planes src[i] [nseq][Hkv][cap] rows of row_bytes[i] (a multiple of 4) to
+ * slots 0.. of dst[i] [nseq][Hkv][dcap], dcap >= keep: the planes of a 4-bit cache, or of an fp32 one. No source
+ * overlaps a destination. kept [nseq][Hkv][keep]: the source slots (-1 past the kept ones); score_out
+ * [nseq][Hkv][dcap]: their scores (0 up to `keep`), ready to accumulate on; len_out [nseq]: min(n, keep).
+ * kept, score_out and len_out may be NULL. max_len: the largest n. */
+#define ORK_B200_EVICT_PLANES 8
+typedef struct ork_b200_evict {
+  const float *score;
+  const int *len;
+  int nseq, Hkv, cap, dcap, max_len, keep, sinks, recent, nplanes;
+  const void *src[ORK_B200_EVICT_PLANES];
+  void *dst[ORK_B200_EVICT_PLANES];
+  int row_bytes[ORK_B200_EVICT_PLANES];
+  int *kept;
+  float *score_out;
+  int *len_out;
+} ork_b200_evict;
+int ork_b200_evict_async(ork_npu *ctx, const ork_b200_evict *e);
+
 /* Column-sharded runs with the gather fused into the matmul (one process per GPU, NVLink peer memory).
  * Rank g of R holds output channels [col0, col0 + ncols) of a weight; its run writes those columns of C
  * into EVERY rank's C buffer ([M][ldc] int32) and signals every rank once per run; a rank that needs C

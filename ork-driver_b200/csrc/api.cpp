@@ -74,7 +74,8 @@ bool err_word_init(int dev) {
   unsigned int *d = nullptr;
   if (cudaHostGetDevicePointer((void **)&d, g_err_host + dev, 0) != cudaSuccess) return false;
   cudaError_t (*set[])(unsigned int *) = {gemv_set_err_word, tc_set_err_word, layer_set_err_word,
-                                          fused_set_err_word, peer_set_err_word};
+                                          fused_set_err_word, peer_set_err_word, attn_set_err_word, kv4_set_err_word,
+                                          evict_set_err_word};
   for (auto f : set)
     if (f(d) != cudaSuccess) return false;
   g_err_ready[dev] = true;
@@ -90,6 +91,7 @@ bool device_error() {
   if (!*w) return false;
   *w = 0u;
   tc_error_flag(true), gemv_error_flag(true), layer_error_flag(true), fused_error_flag(true), peer_error_flag(true);
+  attn_error_flag(true), kv4_error_flag(true), evict_error_flag(true);
   return true;
 }
 
@@ -418,6 +420,7 @@ void ork_npu_free(ork_npu *c) {
     layer_tabs_free(c);
     if (c->dL) cudaFree(c->dL);
     if (c->dX) cudaFree(c->dX);
+    if (c->dW) cudaFree(c->dW);
     if (c->dG) cudaFree(c->dG);
     if (c->dF) cudaFree(c->dF);
     if (c->hP) cudaFreeHost(c->hP);
@@ -610,7 +613,7 @@ int ork_b200_f16_mm_run_async(ork_npu *c, ork_w *w, int M, const ork_f16 *dA, fl
 }
 
 size_t ork_b200_staging_bytes(const ork_npu *c) {
-  return c ? c->capA + c->capC + c->capS + c->capL + c->capX + c->capP : 0;
+  return c ? c->capA + c->capC + c->capS + c->capL + c->capX + c->capP + c->capW : 0;
 }
 
 int ork_b200_reload_tuning(ork_npu *c) {
@@ -628,7 +631,7 @@ int ork_b200_sync(ork_npu *c) {
     return -1;
   }
   if (device_error()) {
-    fprintf(stderr, "[ork] ERROR ork_b200_sync: a kernel reported an error (a bounded wait timed out, or a decode position outside the caches)\n");
+    fprintf(stderr, "[ork] ERROR ork_b200_sync: a kernel reported an error (a bounded wait timed out, or a position, length or row offset outside the caches)\n");
     return -1;
   }
   return 0;

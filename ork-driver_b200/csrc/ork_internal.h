@@ -68,6 +68,9 @@ inline bool gemv_supports(int fmt, int K) { return K > 0 && fmt >= FMT_F16 && fm
 unsigned int gemv_error_flag(bool reset);
 unsigned int layer_error_flag(bool reset);  // layer.cu: a position outside the caches
 unsigned int peer_error_flag(bool reset);   // peers.cu: a peer wait expired
+unsigned int attn_error_flag(bool reset);   // attn.cu: row offsets outside the tensors, a wait that expired
+unsigned int kv4_error_flag(bool reset);    // kv4.cu: a slot or length outside the cache
+unsigned int evict_error_flag(bool reset);  // evict.cu: a length outside the cache
 // Raise a kernel's dynamic shared-memory limit on the current device, once per (kernel, device): the
 // attribute belongs to the device's context, so a process driving several GPUs needs it on each.
 cudaError_t smem_attr(const void *kernel, int bytes);
@@ -77,6 +80,9 @@ cudaError_t tc_set_err_word(unsigned int *p);
 cudaError_t layer_set_err_word(unsigned int *p);
 cudaError_t fused_set_err_word(unsigned int *p);
 cudaError_t peer_set_err_word(unsigned int *p);
+cudaError_t attn_set_err_word(unsigned int *p);
+cudaError_t kv4_set_err_word(unsigned int *p);
+cudaError_t evict_set_err_word(unsigned int *p);
 
 // Grouped (per-K-group scaled) matmul, ork-driver src/npu/core/buf.c:501-520: C[m][n] fp32 = sum over
 // groups g, ascending, of ((float)P_g[m][n] * aScale[m*Sk+g]) * bScale[g*N+n], P_g the exact int32 dot

@@ -19,7 +19,7 @@ ORK_QK_CODEBOOK_NF4 = 1
 _lib = None
 
 # (name, restype, argtypes) for every function declared in include/ork_npu.h and include/ork_b200.h.
-_vp, _i, _sz, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
+_vp, _i, _sz, _f, _ll = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_longlong
 SIGNATURES = [
     ("ork_npu_version", C.c_char_p, []),
     ("ork_pack_format_version", C.c_uint32, []),
@@ -53,6 +53,11 @@ SIGNATURES = [
     ("ork_b200_i8_mm_run_out16_async", _i, [_vp, _vp, _i, _vp, _vp, _i, _i]),
     ("ork_b200_i8_mm_run_ewmul_async", _i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _i]),
     ("ork_i8_npu_ewmul", _i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, C.POINTER(C.c_double)]),
+    ("ork_b200_attn_async", _i, [_vp, _vp]),
+    ("ork_b200_kv4_store_async", _i, [_vp, _vp, _vp, _vp, _i, _i, _ll, _ll, _vp, _vp]),
+    ("ork_b200_kv4_load_async", _i, [_vp, _vp, _vp, _vp, _i, _i, _ll, _ll, _vp, _vp]),
+    ("ork_b200_kv4_attn_async", _i, [_vp, _vp, _vp]),
+    ("ork_b200_evict_async", _i, [_vp, _vp]),
     ("ork_b200_sym_alloc", _vp, [_vp, _sz, _vp]),
     ("ork_b200_sym_free", _i, [_vp, _vp]),
     ("ork_b200_sym_open", _vp, [_vp, _vp]),
@@ -285,6 +290,40 @@ class LayerW(C.Structure):
     """ork_b200_layer_w (include/ork_b200.h): one layer of ork_b200_i8_mm_layers_async."""
     _fields_ = [(n, C.c_void_p) for n in ("wq", "wk", "wv", "wo", "wg", "wu", "wd", "attn_norm", "q_norm",
                                           "ffn_norm", "k_norm", "Kc", "Vc")]
+
+
+# element types of the long-context operators (ORK_B200_F32 / _F16 / _BF16)
+TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+class Attn(C.Structure):
+    """ork_b200_attn (include/ork_b200.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out")] + \
+        [(n, C.c_int) for n in ("type", "nseq", "H", "Hkv", "dk")] + \
+        [(n, C.c_longlong) for n in ("q_ts", "q_hs", "k_ts", "k_hs", "v_ts", "v_hs", "o_ts", "o_hs")] + \
+        [("q_start", C.c_void_p), ("k_start", C.c_void_p)] + \
+        [(n, C.c_int) for n in ("q_rows", "k_rows", "max_q", "max_k")] + \
+        [("scale", C.c_float), ("window", C.c_int), ("sinks", C.c_int)]
+
+
+class KV4(C.Structure):
+    """ork_b200_kv4 (include/ork_b200.h): a 4-bit key/value cache in the caller's device memory."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "kp", "vp")] + [(n, C.c_int) for n in ("nseq", "Hkv", "dk", "cap")]
+
+
+class KV4Attn(C.Structure):
+    """ork_b200_kv4_attn (include/ork_b200.h)."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("type", C.c_int), ("H", C.c_int), ("T", C.c_int),
+                ("q_ts", C.c_longlong), ("q_hs", C.c_longlong), ("len", C.c_void_p), ("max_len", C.c_int),
+                ("scale", C.c_float), ("window", C.c_int), ("sinks", C.c_int), ("wsum", C.c_void_p)]
+
+
+class Evict(C.Structure):
+    """ork_b200_evict (include/ork_b200.h)."""
+    _fields_ = [("score", C.c_void_p), ("len", C.c_void_p)] + \
+        [(n, C.c_int) for n in ("nseq", "Hkv", "cap", "dcap", "max_len", "keep", "sinks", "recent", "nplanes")] + \
+        [("src", C.c_void_p * 8), ("dst", C.c_void_p * 8), ("row_bytes", C.c_int * 8), ("kept", C.c_void_p),
+         ("score_out", C.c_void_p), ("len_out", C.c_void_p)]
 
 
 class Weight:
