@@ -421,6 +421,7 @@ void ork_npu_free(ork_npu *c) {
     if (c->dL) cudaFree(c->dL);
     if (c->dX) cudaFree(c->dX);
     if (c->dW) cudaFree(c->dW);
+    if (c->dK) cudaFree(c->dK);
     if (c->dG) cudaFree(c->dG);
     if (c->dF) cudaFree(c->dF);
     if (c->hP) cudaFreeHost(c->hP);
@@ -613,7 +614,7 @@ int ork_b200_f16_mm_run_async(ork_npu *c, ork_w *w, int M, const ork_f16 *dA, fl
 }
 
 size_t ork_b200_staging_bytes(const ork_npu *c) {
-  return c ? c->capA + c->capC + c->capS + c->capL + c->capX + c->capP + c->capW : 0;
+  return c ? c->capA + c->capC + c->capS + c->capL + c->capX + c->capP + c->capW + c->capK : 0;
 }
 
 int ork_b200_reload_tuning(ork_npu *c) {

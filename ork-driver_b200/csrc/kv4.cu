@@ -14,6 +14,7 @@
 #include "errword.cuh"
 #include "ork_internal.h"
 #include "ork_structs.h"
+#include "sm100.cuh"
 
 namespace orkb {
 
@@ -158,6 +159,48 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(Rows r, E *k, E *
 }
 
 // ---- attention over the cache ----------------------------------------------------------------------------------
+// With s_j, b_j the step and lowest value of token j (per 64 dims g) and c_j its codes,
+//   q . k_j = sum_g s_jg (q_g . c_jg) + b_jg sum(q_g),   out = sum_j p_j v_j = sum_j (p_j s_jg) c_jg + sum_j p_j b_jg,
+// so the codes enter the matrix instructions as integers and are never dequantized. They are the 16-row operand of
+// the instructions (16 tokens of k, then 16 dims of v) and the query rows the 8 columns: a decode step has no more
+// rows than that per kv head, and the other way round half of each product would be padding.
+// First product, mma.m16n8k32 of 8-bit integers: an AND takes four codes out of a word. q is scaled per row to
+// integers below 2^20 and split into three signed bytes; the three products run one after another, the sums shifted
+// left by eight between them, and stay below 2^30: the logits carry q's 20 bits and no other error. (A code in the
+// low bits of an fp16 is an exact subnormal too, and one instruction fewer; but the tensor cores align what they add
+// by the nominal exponents, and the leading zeros cost 6 to 10 of their 24 bits: logits were off by 2^-15.)
+// Second product, mma.m16n8k16 of fp16: there those bits are to spare. A nibble in the low byte of a 16-bit half is
+// the subnormal code * 2^-24 (its low nibble) or code * 2^-20 (its high one); one AND yields two operands, and the
+// scales are taken out of the sums at the end. p * step, rounded to fp16 (11 bits; the output has no more), is
+// transposed between the products with movmatrix; a power of two per warp keeps it in range. For fp32 queries
+// (SPLIT) it is split into an fp16 and the fp16 of what that leaves, 22 bits together, the product runs twice, and
+// all codes are shifted to the top of the mantissa, code * 2^-18.
+// The codes of v are not negative although v has no sign: their sum would grow far above the output that it is to
+// leave after the lowest values' share is added, and the tensor cores truncate what they add. So each stage ends
+// with 8 * sum(p * step) taken out again (the sum by a product with ones, so that it holds the rounded p * step), and
+// v is (c - 8) s + (b + 8 s).
+//
+// A warp owns a run of 16-token units and brings kStageUnits of them at a time into its own ring of shared memory
+// with bulk copies (codes and parameters of k and v, contiguous); no other warp waits on it. The parameters are
+// widened to fp32 once per stage (each token's are needed by four lanes). Softmax is kept online per stage. The warps
+// of a CTA, then the CTAs of a (sequence, kv head, row tile) -- its tokens are split over gridDim.x -- are joined in a
+// fixed order, so results do not depend on timing.
+//
+// Lane layout (r = lane / 4, c = lane % 4). First product: row m of a unit is token (m & 7) / 2 + 4 (m & 1) + 8 (m / 8),
+// contraction quadruples are the dims (e, e + 2, e + 4, e + 6) that one AND leaves, column r is query row r of q's
+// fragment; the accumulators are rows 2 c and 2 c + 1 at the tokens of m = r and r + 8. Second product: contraction pairs are the
+// tokens (c, c + 4) and (c + 8, c + 12), put side by side by a byte permutation; row r of a tile (g, j) is dim
+// 64 g + 8 r + 2 j, row r + 8 the dim after it. This order of the tokens keeps both reads of codes to two-way bank
+// conflicts (64-byte rows; four consecutive tokens where the plain order would read every other one).
+constexpr int kWarps = 4;   // per CTA
+constexpr int kUnit = 16;   // tokens
+constexpr int kStageUnits = 3;
+constexpr int kStageTok = kUnit * kStageUnits;
+constexpr int kRows = 8;    // query rows of a column tile
+// The sums are scaled by 2^-m for an m that only follows the running maximum once that is kRise above it: most
+// stages raise the maximum of some of the eight rows a little, and scaling the accumulators for that was a fifth of
+// the instructions. Weights reach 2^kRise; times the largest scaled step (64) they stay below fp16's 65504.
+constexpr float kRise = 5.0f;
 
 struct Attn4 {
   const uint8_t *kc, *vc;
@@ -167,88 +210,754 @@ struct Attn4 {
   const int *len;
   float scale;
   float *wsum;
-  float2 *stat;  // softmax maximum and sum of every row, for wsum
+  int splits, tiles, prow;  // token splits; row tiles, and their rows in all
+  bool qvec;          // q's rows are 16-byte aligned
+  bool join;          // the last CTA of an item joins its splits
+  unsigned int *done; // [nseq * Hkv * tiles] counts of finished splits, zero between launches
+  int vis;            // most tokens that a row range can see, a multiple of kUnit (x's row stride)
+  float *po;          // partial outputs [nseq][Hkv][prow][splits][dk], normalised by nothing
+  float2 *pml;        // their maxima (log2 units) and sums [nseq][Hkv][prow][splits]
+  float *x;           // logits in log2 units [nseq][Hkv][prow][vis], kept for wsum
 };
 
-// the number of tokens of sequence s; -1 (reported) where it cannot be
+// The visible tokens of a sequence as 16-token units: su units of sinks from token 0 on, then the window's.
+struct Units {
+  int n, su, lo, all;  // tokens held; sink units; first unit of the window; units in all
+};
+__device__ __forceinline__ Units units_of(const Attn4 &a, int n) {
+  Units u;
+  u.n = n;
+  const int first = a.window && n - a.T - a.window + 1 > 0 ? n - a.T - a.window + 1 : 0;
+  u.lo = first / kUnit;
+  u.su = min((a.sinks + kUnit - 1) / kUnit, u.lo);
+  u.all = u.su + (n + kUnit - 1) / kUnit - u.lo;
+  return u;
+}
+__device__ __forceinline__ int token_of(const Units &u, int unit) {
+  return (unit < u.su ? unit : unit - u.su + u.lo) * kUnit;
+}
+
+// the number of tokens of sequence s; 0 (reported) where it cannot be
 __device__ __forceinline__ int seq_len(const Attn4 &a, int s) {
   const int n = a.len[s];
-  if (n >= 0 && n <= a.max_len && n <= a.cap) return n;
+  if (n >= 0 && n <= a.max_len) return n;
   if (threadIdx.x == 0) kv4_error();
-  return -1;
+  return 0;
 }
 __device__ __forceinline__ bool visible(const Attn4 &a, int p, int j) {
   return j <= p && (a.window == 0 || j > p - a.window || j < a.sinks);
 }
 
+// d += a b: fp16, 16 x 8 x 16; mma0: d = a b. mma_i8: unsigned times signed bytes, 16 x 8 x 32
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma_i8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_i80(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
+// byte i of each of four words
+__device__ __forceinline__ uint32_t bytes_of(const int (&w)[4], int i) {
+  const uint32_t sel = (uint32_t)(i | (i + 4) << 4);
+  return __byte_perm(__byte_perm((uint32_t)w[0], (uint32_t)w[1], sel), __byte_perm((uint32_t)w[2], (uint32_t)w[3], sel), 0x5410);
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // an 8 x 8 tile of 16-bit values
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+// x as fp16 pairs: the rounded values, and what they leave
+__device__ __forceinline__ void split2(float2 x, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __float22half2_rn(x);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x.x - f.x, x.y - f.y);
+  hi = *reinterpret_cast<const uint32_t *>(&h);
+  lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+__device__ __forceinline__ float quad_max(float v) {  // over c
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+__device__ __forceinline__ float col_max(float v) {  // over r
+  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float col_sum(float v) {
+  for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// the power of two 2^e
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
 template <int DK>
-__device__ __forceinline__ float value4(const uint8_t *codes, const __half *par, size_t tok, int d) {
-  const uint8_t b = codes[tok * (DK / 2) + d / 2];
-  const __half *p = par + (tok * (DK / kGroup) + d / kGroup) * 2;
-  return (float)((d & 1) ? b >> 4 : b & 15) * __half2float(p[0]) + __half2float(p[1]);
-}
+struct Stage {  // one ring slot of a warp
+  uint8_t k[kStageTok * DK / 2], v[kStageTok * DK / 2];
+  __half2 kp[kStageTok * (DK / kGroup)], vp[kStageTok * (DK / kGroup)];
+};
+// A stage's parameters in fp32: of each token the steps of its groups, then the lowest values (k), or the scaled steps
+// and b + 8 s (v).
+template <int DK>
+struct Wide {
+  float k[kStageTok][2 * (DK / kGroup)], v[kStageTok][2 * (DK / kGroup)];
+};
+template <int DK>
+constexpr int kStages = DK == 128 ? 2 : 4;
+// CTAs that an SM holds: with both halves of fp32 queries, or two column tiles, the registers of three would spill
+template <class E, int DK, int NT>
+constexpr int kCtas = DK == 128 && (NT == 2 || sizeof(E) == 4) ? 2 : 3;
+template <int DK>
+constexpr int kAttnSmem = kWarps * (kStages<DK> * ((int)sizeof(Stage<DK>) + 8) + (int)sizeof(Wide<DK>));
 
-// One warp per (sequence, token, query head); lane l holds dims l + 32 u.
-template <class E, int DK>
-__global__ void __launch_bounds__(32) kv4_attn_kernel(Attn4 a, const E *__restrict__ q, E *__restrict__ out) {
-  constexpr int PER = DK / 32;
-  const int lane = threadIdx.x, h = blockIdx.x % a.H, st = blockIdx.x / a.H, s = st / a.T, t = st % a.T;
-  const int n = seq_len(a, s), p = n - a.T + t, kvh = h / (a.H / a.Hkv);
-  float qv[PER], o[PER] = {}, m = -INFINITY, l = 0.0f;
-  for (int u = 0; u < PER; u++) qv[u] = to_f32(q[(long long)st * a.q_ts + (long long)h * a.q_hs + lane + 32 * u]) * a.scale;
-  for (int j = 0; n >= 0 && j <= p; j++) {
-    if (!visible(a, p, j)) continue;
-    const size_t tok = ((size_t)s * a.Hkv + kvh) * a.cap + j;
-    float x = 0.0f;
-    for (int u = 0; u < PER; u++) x += qv[u] * value4<DK>(a.kc, a.kp, tok, lane + 32 * u);
-    for (int k = 16; k; k >>= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
-    const float mn = fmaxf(m, x), c = m == mn ? 1.0f : __expf(m - mn), w = x == mn ? 1.0f : expf(x - mn);
-    l = l * c + w;
-    for (int u = 0; u < PER; u++) o[u] = o[u] * c + w * value4<DK>(a.vc, a.vp, tok, lane + 32 * u);
-    m = mn;
+template <int N>
+__device__ __forceinline__ void load_pars(const float *p, float (&x)[N]) {
+  if constexpr (N == 4) {
+    const float4 v = *reinterpret_cast<const float4 *>(p);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const float2 v = *reinterpret_cast<const float2 *>(p);
+    x[0] = v.x, x[1] = v.y;
   }
-  for (int u = 0; u < PER; u++)
-    out[((long long)st * a.H + h) * DK + lane + 32 * u] = from_f32<E>(l > 0.0f ? o[u] / l : (l == 0.0f ? 0.0f : l));
-  if (a.wsum && lane == 0) a.stat[(size_t)st * a.H + h] = make_float2(m, l);
+}
+template <int N>
+__device__ __forceinline__ void store_pars(float *p, const float (&x)[N]) {
+  if constexpr (N == 4) *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  else *reinterpret_cast<float2 *>(p) = make_float2(x[0], x[1]);
+}
+// the NG parameter pairs (step, lowest) of a token
+template <int NG>
+__device__ __forceinline__ void token_pars(const __half2 *p, float2 (&x)[NG]) {
+  if constexpr (NG == 2) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    x[0] = __half22float2(*reinterpret_cast<const __half2 *>(&v.x));
+    x[1] = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
+  } else {
+    x[0] = __half22float2(*p);
+  }
 }
 
-// wsum: one warp per (sequence, kv head, key), the rows in order.
-template <class E, int DK>
-__global__ void __launch_bounds__(256) kv4_wsum_kernel(Attn4 a, const E *__restrict__ q) {
-  constexpr int PER = DK / 32;
-  const int lane = threadIdx.x & 31, s = blockIdx.y / a.Hkv, kvh = blockIdx.y % a.Hkv, G = a.H / a.Hkv;
-  const int j = blockIdx.x * 8 + (threadIdx.x >> 5), n = seq_len(a, s);
-  if (j >= n) return;
-  const size_t tok = ((size_t)s * a.Hkv + kvh) * a.cap + j;
-  float kv[PER], sum = 0.0f;
-  for (int u = 0; u < PER; u++) kv[u] = value4<DK>(a.kc, a.kp, tok, lane + 32 * u) * a.scale;
-  for (int t = 0; t < a.T; t++) {
-    if (!visible(a, n - a.T + t, j)) continue;
-    for (int g = 0; g < G; g++) {
-      const int st = s * a.T + t, h = kvh * G + g;
-      float x = 0.0f;
-      for (int u = 0; u < PER; u++) x += kv[u] * to_f32(q[(long long)st * a.q_ts + (long long)h * a.q_hs + lane + 32 * u]);
-      for (int k = 16; k; k >>= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
-      const float2 ml = a.stat[(size_t)st * a.H + h];
-      sum += expf(x - ml.x) / ml.y;
+template <int DK>
+__device__ __forceinline__ void load_stage(const Attn4 &a, size_t base, const Units &u, int unit, int cnt, Stage<DK> *st,
+                                           uint32_t bar, int lane) {
+  constexpr int NG = DK / kGroup;
+  const size_t tok = base + (size_t)token_of(u, unit);
+  const uint32_t cb = (uint32_t)cnt * kUnit * (DK / 2), pb = (uint32_t)cnt * kUnit * NG * 4;
+  if (lane == 0) sm100::bar_expect(bar, 2 * cb + 2 * pb);
+  __syncwarp();
+  if (lane == 0) sm100::bulk_load(sm100::smem_addr(st->k), a.kc + tok * (DK / 2), cb, bar);
+  else if (lane == 1) sm100::bulk_load(sm100::smem_addr(st->kp), a.kp + tok * NG * 2, pb, bar);
+  else if (lane == 2) sm100::bulk_load(sm100::smem_addr(st->v), a.vc + tok * (DK / 2), cb, bar);
+  else if (lane == 3) sm100::bulk_load(sm100::smem_addr(st->vp), a.vp + tok * NG * 2, pb, bar);
+}
+
+// NT column tiles of kRows query rows share every operand made from the codes.
+template <class E, int DK, int NT, bool WS>
+__global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel(const Attn4 a, const E *__restrict__ q, E *__restrict__ out) {
+  constexpr int NG = DK / kGroup, NST = kStages<DK>, TR = NT * kRows;
+  constexpr bool SPLIT = sizeof(E) == 4;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // known to be the same for the whole warp
+  const int split = blockIdx.x % a.splits, th = blockIdx.x / a.splits, kvh = th / a.tiles, tile = th % a.tiles;
+  const int s = blockIdx.y, G = a.H / a.Hkv, rows = a.T * G;
+  Stage<DK> *ring = reinterpret_cast<Stage<DK> *>(smem) + warp * NST;
+  Wide<DK> *wide = reinterpret_cast<Wide<DK> *>(smem + kWarps * NST * sizeof(Stage<DK>)) + warp;
+  const uint32_t bars = sm100::smem_addr(smem + kWarps * (NST * sizeof(Stage<DK>) + sizeof(Wide<DK>))) + warp * NST * 8;
+  if (lane < NST) sm100::bar_init(bars + 8 * lane, 1);
+  sm100::bar_init_fence();
+  __syncwarp();
+
+  const int n = seq_len(a, s);
+  const Units u = units_of(a, n);
+  const int cu0 = (int)((long long)u.all * split / a.splits), cu1 = (int)((long long)u.all * (split + 1) / a.splits);
+  const int u0 = cu0 + (cu1 - cu0) * warp / kWarps, u1 = cu0 + (cu1 - cu0) * (warp + 1) / kWarps;
+  const size_t base = ((size_t)s * a.Hkv + kvh) * a.cap;
+  // a stage ends at the jump from the sinks to the window
+  auto count = [&](int unit) { return min(min(kStageUnits, u1 - unit), unit < u.su ? u.su - unit : kStageUnits); };
+  int next = u0;  // first unit not yet requested
+#pragma unroll
+  for (int i = 0; i < NST; i++)
+    if (next < u1) {
+      const int cnt = count(next);
+      load_stage<DK>(a, base, u, next, cnt, ring + i, bars + 8 * i, lane);
+      next += cnt;
+    }
+
+  // q of row r of each tile: byte 2 - d of the integers of the lane's words i, even dims then odd ones
+  uint32_t qd[NT][3][NG][2][2];
+  float fs[NT][2], qs[NT][NG][2];  // of the rows 2 c and 2 c + 1 that the accumulators hold
+#pragma unroll
+  for (int y = 0; y < NT; y++) {
+    const int row = tile * TR + y * kRows + r;
+    const bool live = row < rows;
+    const E *qr = q + ((long long)s * a.T + row / G) * a.q_ts + (long long)(kvh * G + row % G) * a.q_hs;
+    float x[NG][16], mx = 0.0f;
+    bool fin = true;
+#pragma unroll
+    for (int g = 0; g < NG; g++)
+#pragma unroll
+      for (int i = 0; i < 16; i += 8) {
+        float w[8] = {};
+        if (live) load8<E>(qr + 64 * g + 16 * c + i, a.qvec, w);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          x[g][i + j] = w[j];
+          mx = fmaxf(mx, fabsf(w[j]));
+          fin = fin && fabsf(w[j]) <= 3.402823466e38f;
+        }
+      }
+    mx = quad_max(mx);
+    const unsigned quad = 15u << (lane & 28);
+    fin = (__ballot_sync(0xffffffffu, fin) & quad) == quad;
+    const int e = fin ? max(-100, min(100, 146 - (int)(__float_as_uint(mx) >> 23))) : 0;
+    const float up = pow2(e), f = fin ? a.scale * 1.4426950408889634f * pow2(-e) : __int_as_float(0x7fc00000);
+    float sums[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+      int w[16], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        w[i] = fin ? __float2int_rn(x[g][i] * up) : 0;
+        sum += w[i];
+        w[i] += 0x808080;  // bytes of 128 + digit
+      }
+      sums[g] = quad_sum((float)sum) * f;
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int odd = 0; odd < 2; odd++) {
+          const int w4[4] = {w[8 * i + odd], w[8 * i + 2 + odd], w[8 * i + 4 + odd], w[8 * i + 6 + odd]};
+#pragma unroll
+          for (int d = 0; d < 3; d++) qd[y][d][g][i][odd] = bytes_of(w4, 2 - d) ^ 0x80808080u;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int from = (2 * c + i) * 4;
+      fs[y][i] = __shfl_sync(0xffffffffu, f, from);
+#pragma unroll
+      for (int g = 0; g < NG; g++) qs[y][g][i] = __shfl_sync(0xffffffffu, sums[g], from);
     }
   }
-  if (lane == 0) a.wsum[tok] += sum;
+
+  float o[NT][NG][4][4], z[NT][NG][2], l[NT][2], mrow[NT][2];
+#pragma unroll
+  for (int y = 0; y < NT; y++)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      l[y][i] = 0.0f, mrow[y][i] = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < NG; g++) {
+        z[y][g][i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[y][g][j][i] = o[y][g][j][i + 2] = 0.0f;
+      }
+    }
+  float vs = 1.0f, vlim = 0.0f;  // scale of p * step, and the largest step it is good for (the first stage sets both)
+  bool ok = true;
+  int slot = 0;
+  uint32_t parity = 0;
+  for (int unit = u0; unit < u1;) {
+    const int cnt = count(unit), tok0 = token_of(u, unit), tok1 = tok0 + cnt * kUnit;
+    const Stage<DK> *st = ring + slot;
+    ok = sm100::bar_wait(bars + 8 * slot, parity);
+    if (!ok) break;
+    // every token of the stage visible to every row?
+    const bool whole = cnt == kStageUnits && tok1 <= n - a.T + 1 && (a.window == 0 || tok0 > n - 1 - a.window || tok1 <= a.sinks);
+    constexpr int PT = (kStageTok + 31) / 32;
+    float vpar[PT][2 * NG], top = 0.0f;  // of the tokens that this lane widens
+#pragma unroll
+    for (int i = 0; i < PT; i++) {
+      const int tk = lane + 32 * i, j = tok0 + tk;
+      if (kStageTok % 32 == 0 || tk < kStageTok) {
+        float2 kf[NG], vf[NG];
+        token_pars<NG>(st->kp + tk * NG, kf);
+        token_pars<NG>(st->vp + tk * NG, vf);
+        if (!whole) {
+          const bool seen = tk < cnt * kUnit && j < n && (a.window == 0 || j > n - a.T - a.window || j < a.sinks);
+#pragma unroll
+          for (int g = 0; g < NG; g++)
+            if (!seen) kf[g] = vf[g] = make_float2(0.0f, 0.0f);
+          // a value that is not a number reaches the rows that see the token through its logit: 0 * NaN would
+          // reach them all
+          bool bad = false;
+#pragma unroll
+          for (int g = 0; g < NG; g++) bad = bad || !(fabsf(vf[g].x) <= 1e6f) || !(fabsf(vf[g].y) <= 1e6f);
+          if (bad) {
+#pragma unroll
+            for (int g = 0; g < NG; g++) kf[g] = both(__int_as_float(0x7fc00000)), vf[g] = both(0.0f);
+          }
+        }
+        float kpar[2 * NG];
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+          kpar[g] = kf[g].x, kpar[NG + g] = kf[g].y;
+          vpar[i][g] = vf[g].x, vpar[i][NG + g] = fmaf(8.0f, vf[g].x, vf[g].y);
+          top = fmaxf(top, vf[g].x);
+        }
+        store_pars(wide->k[tk], kpar);
+      }
+    }
+    if (__any_sync(0xffffffffu, top > vlim)) {  // rare: steps rarely grow 32-fold
+      for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      // the largest step becomes 1 .. 2
+      const float ns = pow2(min(127 - (int)(__float_as_uint(top) >> 23), 100)), k = vlim > 0.0f ? ns / vs : 0.0f;
+      vs = ns;
+      vlim = 64.0f / ns;
+#pragma unroll
+      for (int y = 0; y < NT; y++)
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[y][g][j][i] *= k;
+    }
+#pragma unroll
+    for (int i = 0; i < PT; i++) {
+      const int tk = lane + 32 * i;
+      if (kStageTok % 32 == 0 || tk < kStageTok) {
+#pragma unroll
+        for (int g = 0; g < NG; g++) vpar[i][g] *= vs;
+        store_pars(wide->v[tk], vpar[i]);
+      }
+    }
+    __syncwarp();
+
+    float x[NT][kStageUnits][4];  // logits of row 2 c + i % 2 at the token of m = r + 8 (i / 2), in log2 units
+    const int mt = (r >> 1) + 4 * (r & 1);
+#pragma unroll
+    for (int w = 0; w < kStageUnits; w++) {  // units past cnt hold old codes, and steps of zero
+      int acc[NT][NG][4];
+#pragma unroll
+      for (int g = 0; g < NG; g++) {
+        const uint8_t *kr = st->k + (kUnit * w + mt) * (DK / 2) + g * 32 + c * 8;
+        const uint2 k0 = *reinterpret_cast<const uint2 *>(kr), k1 = *reinterpret_cast<const uint2 *>(kr + 8 * (DK / 2));
+        const uint32_t af[2][4] = {
+            {k0.x & 0x0f0f0f0fu, k1.x & 0x0f0f0f0fu, (k0.x >> 4) & 0x0f0f0f0fu, (k1.x >> 4) & 0x0f0f0f0fu},
+            {k0.y & 0x0f0f0f0fu, k1.y & 0x0f0f0f0fu, (k0.y >> 4) & 0x0f0f0f0fu, (k1.y >> 4) & 0x0f0f0f0fu}};
+#pragma unroll
+        for (int y = 0; y < NT; y++)
+#pragma unroll
+          for (int d = 0; d < 3; d++) {
+            if (d == 0) mma_i80(acc[y][g], af[0], qd[y][d][g][0][0], qd[y][d][g][0][1]);
+            else {
+#pragma unroll
+              for (int i = 0; i < 4; i++) acc[y][g][i] <<= 8;
+              mma_i8(acc[y][g], af[0], qd[y][d][g][0][0], qd[y][d][g][0][1]);
+            }
+            mma_i8(acc[y][g], af[1], qd[y][d][g][1][0], qd[y][d][g][1][1]);
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float par[2 * NG];
+        load_pars(wide->k[kUnit * w + 8 * h + mt], par);
+#pragma unroll
+        for (int y = 0; y < NT; y++)
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            float d = (float)acc[y][0][2 * h + i] * par[0], b = par[NG] * qs[y][0][i];
+            if constexpr (NG == 2) {
+              d = fmaf((float)acc[y][1][2 * h + i], par[1], d);
+              b = fmaf(par[NG + 1], qs[y][1][i], b);
+            }
+            x[y][w][2 * h + i] = fmaf(d, fs[y][i], b);
+          }
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int y = 0; y < NT; y++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const int p = n - a.T + (tile * TR + y * kRows + 2 * c + i) / G;  // the row's position
+#pragma unroll
+          for (int w = 0; w < kStageUnits; w++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+              if (w >= cnt || !visible(a, p, tok0 + kUnit * w + 8 * h + mt)) x[y][w][2 * h + i] = -INFINITY;
+        }
+    }
+    if constexpr (WS) {
+#pragma unroll
+      for (int y = 0; y < NT; y++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          float *xr = a.x + (((size_t)s * a.Hkv + kvh) * a.prow + tile * TR + y * kRows + 2 * c + i) * a.vis +
+                      (size_t)unit * kUnit + mt;
+#pragma unroll
+          for (int w = 0; w < kStageUnits; w++)
+            if (w < cnt) xr[kUnit * w] = x[y][w][i], xr[kUnit * w + 8] = x[y][w][2 + i];
+        }
+    }
+    float mx[NT][2];
+    bool rise = false;
+#pragma unroll
+    for (int y = 0; y < NT; y++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        mx[y][i] = fmaxf(x[y][0][i], x[y][0][2 + i]);
+#pragma unroll
+        for (int w = 1; w < kStageUnits; w++) mx[y][i] = fmaxf(mx[y][i], fmaxf(x[y][w][i], x[y][w][2 + i]));
+        rise = rise || mx[y][i] > mrow[y][i] + kRise;
+      }
+    if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+      for (int y = 0; y < NT; y++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const float m = fmaxf(mrow[y][i], col_max(mx[y][i])), k = mrow[y][i] == m ? 1.0f : sm100::ex2(mrow[y][i] - m);
+          mrow[y][i] = m;
+          l[y][i] *= k;
+#pragma unroll
+          for (int g = 0; g < NG; g++) {
+            z[y][g][i] *= k;
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[y][g][j][i] *= k, o[y][g][j][i + 2] *= k;
+          }
+        }
+    }
+    float sum[NT][NG][4];  // of p * step, rows 2 c and 2 c + 1 (twice)
+    float mu[NT][2];
+#pragma unroll
+    for (int y = 0; y < NT; y++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) mu[y][i] = mrow[y][i] == -INFINITY ? 0.0f : mrow[y][i];
+#pragma unroll
+    for (int w = 0; w < kStageUnits; w++) {
+      uint32_t ph[NT][NG][2], pl[SPLIT ? NT : 1][NG][2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float par[2 * NG];
+        load_pars(wide->v[kUnit * w + 8 * h + mt], par);
+#pragma unroll
+        for (int y = 0; y < NT; y++) {
+          float e[2], ps[NG][2];
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            e[i] = sm100::ex2(x[y][w][2 * h + i] - mu[y][i]);
+            l[y][i] += e[i];
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+              ps[g][i] = e[i] * par[g];
+              z[y][g][i] = fmaf(e[i], par[NG + g], z[y][g][i]);
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < NG; g++) {
+            if constexpr (SPLIT) {
+              uint32_t lo;
+              split2(make_float2(ps[g][0], ps[g][1]), ph[y][g][h], lo);
+              pl[y][g][h] = transpose8(lo);
+            } else {
+              const __half2 hp = __floats2half2_rn(ps[g][0], ps[g][1]);
+              ph[y][g][h] = *reinterpret_cast<const uint32_t *>(&hp);
+            }
+            ph[y][g][h] = transpose8(ph[y][g][h]);
+          }
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < NG; g++) {
+        const uint32_t one[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+        for (int y = 0; y < NT; y++) {
+          if (w == 0) mma0(sum[y][g], one, ph[y][g][0], ph[y][g][1]);
+          else mma(sum[y][g], one, ph[y][g][0], ph[y][g][1]);
+          if constexpr (SPLIT) mma(sum[y][g], one, pl[y][g][0], pl[y][g][1]);
+        }
+        uint32_t wv[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          wv[k] = *reinterpret_cast<const uint32_t *>(st->v + (kUnit * w + 4 * k + c) * (DK / 2) + g * 32 + r * 4);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {  // dims 2 j and 2 j + 1 of the lane's eight
+          const uint32_t sel = j & 2 ? 0x7632u : 0x5410u;
+          const uint32_t b0 = __byte_perm(wv[0], wv[1], sel), b1 = __byte_perm(wv[2], wv[3], sel);
+          uint32_t af[4];
+          if constexpr (SPLIT) {  // to bits 6 .. 9
+            af[0] = (j & 1 ? b0 >> 2 : b0 << 6) & 0x03c003c0u, af[1] = (j & 1 ? b0 >> 6 : b0 << 2) & 0x03c003c0u;
+            af[2] = (j & 1 ? b1 >> 2 : b1 << 6) & 0x03c003c0u, af[3] = (j & 1 ? b1 >> 6 : b1 << 2) & 0x03c003c0u;
+          } else {
+            const uint32_t s0 = j & 1 ? b0 >> 8 : b0, s1 = j & 1 ? b1 >> 8 : b1;
+            af[0] = s0 & 0x000f000fu, af[1] = s0 & 0x00f000f0u, af[2] = s1 & 0x000f000fu, af[3] = s1 & 0x00f000f0u;
+          }
+#pragma unroll
+          for (int y = 0; y < NT; y++) {
+            mma(o[y][g][j], af, ph[y][g][0], ph[y][g][1]);
+            if constexpr (SPLIT) mma(o[y][g][j], af, pl[y][g][0], pl[y][g][1]);
+          }
+        }
+      }
+    }
+    // take 8 * sum(p * step) out again, in the codes' units
+#pragma unroll
+    for (int y = 0; y < NT; y++)
+#pragma unroll
+      for (int g = 0; g < NG; g++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) o[y][g][j][i] = fmaf(sum[y][g][i & 1], SPLIT ? -0x1p-15f : i & 2 ? -0x1p-17f : -0x1p-21f, o[y][g][j][i]);
+    unit += cnt;
+    __syncwarp();  // every lane has read the slot
+    if (next < u1) {
+      const int more = count(next);
+      load_stage<DK>(a, base, u, next, more, ring + slot, bars + 8 * slot, lane);
+      next += more;
+    }
+    if (++slot == NST) slot = 0, parity ^= 1;
+  }
+  if (!ok && lane == 0) kv4_error();
+
+  // ---- the warps' results, then the CTA's
+  sm100::dependents_launch();
+  constexpr int LDO = DK + 4;
+  float *so = reinterpret_cast<float *>(smem);                        // [kWarps][TR][LDO]
+  float2 *sml = reinterpret_cast<float2 *>(so + kWarps * TR * LDO);   // [kWarps][TR]
+  static_assert(kWarps * TR * (LDO * 4 + 8) + 4 <= kWarps * NST * (int)sizeof(Stage<DK>), "the rings hold it");
+  __syncthreads();  // the rings are idle (a warp whose wait gave up has reported it)
+  const float back = (SPLIT ? 0x1p18f : 0x1p24f) / vs, back1 = SPLIT ? back : back * 0.0625f;
+#pragma unroll
+  for (int y = 0; y < NT; y++)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int rr = warp * TR + y * kRows + 2 * c + i;
+      const float ls = col_sum(l[y][i]);
+      if (r == 0) sml[rr] = make_float2(mrow[y][i], ls);
+#pragma unroll
+      for (int g = 0; g < NG; g++) {
+        const float zz = col_sum(z[y][g][i]);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          v[2 * j] = fmaf(o[y][g][j][i], back, zz), v[2 * j + 1] = fmaf(o[y][g][j][i + 2], back1, zz);
+        float4 *dst = reinterpret_cast<float4 *>(so + rr * LDO + 64 * g + 8 * r);
+        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    }
+  __syncthreads();
+  constexpr int PER = 8;  // consecutive dims of one row
+  for (int at = threadIdx.x; at < TR * DK / PER; at += 32 * kWarps) {
+    const int rr = at * PER / DK, d0 = at * PER % DK, row = tile * TR + rr;
+    if (row >= rows) break;
+    float m = -INFINITY, sum = 0.0f, v[PER] = {};
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) m = fmaxf(m, sml[w * TR + rr].x);
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+      const float2 ml = sml[w * TR + rr];
+      const float k = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : sm100::ex2(ml.x - m);
+      sum = fmaf(k, ml.y, sum);
+      if (k != 0.0f)
+#pragma unroll
+        for (int i = 0; i < PER; i++) v[i] = fmaf(k, so[(w * TR + rr) * LDO + d0 + i], v[i]);
+    }
+    const size_t pr = (((size_t)s * a.Hkv + kvh) * a.prow + row) * a.splits + split;
+    if ((WS || a.splits > 1) && d0 == 0) a.pml[pr] = make_float2(m, sum);
+    if (a.splits > 1) {
+      float4 *dst = reinterpret_cast<float4 *>(a.po + pr * DK + d0);
+      dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+      dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      E *dst = out + (((long long)s * a.T + row / G) * a.H + kvh * G + row % G) * DK + d0;
+#pragma unroll
+      for (int i = 0; i < PER; i++) dst[i] = from_f32<E>(sum == 0.0f ? 0.0f : v[i] / sum);
+    }
+  }
+  if (!a.join) return;
+  // few splits: the last CTA to finish joins them, in their order (more go to kv4_join_kernel, a CTA per row)
+  unsigned int *flag = reinterpret_cast<unsigned int *>(sml + kWarps * TR);
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) *flag = atomicInc(a.done + ((size_t)s * a.Hkv + kvh) * a.tiles + tile, a.splits - 1);
+  __syncthreads();
+  if (*flag != (unsigned int)a.splits - 1) return;
+  __threadfence();
+  for (int at = threadIdx.x; at < TR * DK / PER; at += 32 * kWarps) {
+    const int rr = at * PER / DK, d0 = at * PER % DK, row = tile * TR + rr;
+    if (row >= rows) break;
+    const size_t pr = (((size_t)s * a.Hkv + kvh) * a.prow + row) * a.splits;
+    float m = -INFINITY, sum = 0.0f, v[PER] = {};
+    for (int i = 0; i < a.splits; i++) m = fmaxf(m, __ldcg(&a.pml[pr + i].x));
+#pragma unroll 4
+    for (int i = 0; i < a.splits; i++) {
+      const float2 ml = __ldcg(a.pml + pr + i);
+      const float4 *po = reinterpret_cast<const float4 *>(a.po + (pr + i) * DK + d0);
+      const float4 p0 = __ldcg(po), p1 = __ldcg(po + 1);
+      const float k = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : sm100::ex2(ml.x - m);
+      sum = fmaf(k, ml.y, sum);
+      if (k != 0.0f) {
+        v[0] = fmaf(k, p0.x, v[0]), v[1] = fmaf(k, p0.y, v[1]), v[2] = fmaf(k, p0.z, v[2]), v[3] = fmaf(k, p0.w, v[3]);
+        v[4] = fmaf(k, p1.x, v[4]), v[5] = fmaf(k, p1.y, v[5]), v[6] = fmaf(k, p1.z, v[6]), v[7] = fmaf(k, p1.w, v[7]);
+      }
+    }
+    E *dst = out + (((long long)s * a.T + row / G) * a.H + kvh * G + row % G) * DK + d0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) dst[i] = from_f32<E>(sum == 0.0f ? 0.0f : v[i] / sum);
+  }
 }
 
+// Joins the splits of one row (the first `joins` blocks of x) and adds to wsum (the others, kSumTok tokens of one kv
+// head each): wsum[j] += sum over the rows of 2^(x_j - m) / l.
+constexpr int kJoinThreads = 128;
+constexpr int kSumTok = 8 * kJoinThreads;
+template <class E, int DK, bool WS>
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Attn4 a, E *__restrict__ out, int joins) {
+  constexpr int NW = kJoinThreads / 32, PER = DK / 32;
+  __shared__ float2 sml[NW];
+  __shared__ float so[NW][DK];
+  sm100::dependency_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.H / a.Hkv, rows = a.T * G, s = blockIdx.y;
+  if ((int)blockIdx.x < joins) {
+    const int kvh = blockIdx.x / rows, row = blockIdx.x % rows;
+    const size_t pr = (((size_t)s * a.Hkv + kvh) * a.prow + row) * a.splits;
+    float m = -INFINITY, l = 0.0f, v[PER] = {};
+    for (int i0 = 32 * warp; i0 < a.splits; i0 += 32 * NW) {  // lane i: split i0 + i
+      const float2 ml = i0 + lane < a.splits ? a.pml[pr + i0 + lane] : make_float2(-INFINITY, 0.0f);
+      float mn = ml.x;
+      for (int off = 16; off; off >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+      mn = fmaxf(mn, m);
+      const float was = m == mn ? 1.0f : sm100::ex2(m - mn);
+      const float k = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : sm100::ex2(ml.x - mn);
+      m = mn;
+      l = fmaf(k, ml.y, l * was);
+#pragma unroll
+      for (int d = 0; d < PER; d++) v[d] *= was;
+      const int cnt = min(32, a.splits - i0);
+#pragma unroll 16
+      for (int i = 0; i < cnt; i++) {
+        const float ki = __shfl_sync(0xffffffffu, k, i);
+        const float *po = a.po + (pr + i0 + i) * DK + PER * lane;
+#pragma unroll
+        for (int d = 0; d < PER; d++) {
+          const float x = po[d];
+          if (ki != 0.0f) v[d] = fmaf(ki, x, v[d]);
+        }
+      }
+    }
+    for (int off = 16; off; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    if (lane == 0) sml[warp] = make_float2(m, l);
+#pragma unroll
+    for (int d = 0; d < PER; d++) so[warp][PER * lane + d] = v[d];
+    __syncthreads();
+    if ((int)threadIdx.x < DK) {
+      float mm = -INFINITY, sum = 0.0f, x = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; w++) mm = fmaxf(mm, sml[w].x);
+#pragma unroll
+      for (int w = 0; w < NW; w++) {
+        const float k = sml[w].x == -INFINITY && sml[w].y == 0.0f ? 0.0f : sm100::ex2(sml[w].x - mm);
+        sum = fmaf(k, sml[w].y, sum);
+        if (k != 0.0f) x = fmaf(k, so[w][threadIdx.x], x);
+      }
+      out[(((long long)s * a.T + row / G) * a.H + kvh * G + row % G) * DK + threadIdx.x] = from_f32<E>(sum == 0.0f ? 0.0f : x / sum);
+    }
+    return;
+  }
+  if constexpr (WS) {
+    constexpr int CH = 512, PT = kSumTok / kJoinThreads;  // rows at a time, tokens a thread
+    __shared__ float stat[CH];                            // m + log2 l
+    const int per = (a.vis + kSumTok - 1) / kSumTok, at = blockIdx.x - joins, kvh = at / per;
+    const Units u = units_of(a, seq_len(a, s));
+    const int i0 = at % per * kSumTok, live = u.all * kUnit;
+    if (i0 >= live) return;
+    const size_t pr = ((size_t)s * a.Hkv + kvh) * a.prow;
+    float sum[PT] = {};
+    for (int r0 = 0; r0 < rows; r0 += CH) {
+      const int r1 = min(rows, r0 + CH);
+      if (r0) __syncthreads();
+      for (int row = r0 + warp; row < r1; row += NW) {
+        const float2 *ml = a.pml + (pr + row) * a.splits;
+        float m = -INFINITY, l = 0.0f;
+        for (int i = lane; i < a.splits; i += 32) {
+          const float2 x = ml[i];
+          const float mn = fmaxf(m, x.x);
+          if (x.x != -INFINITY || x.y != 0.0f) l = fmaf(sm100::ex2(x.x - mn), x.y, m == mn ? l : l * sm100::ex2(m - mn));
+          m = mn;
+        }
+        for (int off = 16; off; off >>= 1) {
+          const float mo = __shfl_xor_sync(0xffffffffu, m, off), lo = __shfl_xor_sync(0xffffffffu, l, off), mn = fmaxf(m, mo);
+          l = (m == mn ? l : l * sm100::ex2(m - mn)) + (mo == mn ? lo : lo * sm100::ex2(mo - mn));
+          m = mn;
+        }
+        if (lane == 0) stat[row - r0] = m == -INFINITY ? (l == 0.0f ? 0.0f : l) : m + log2f(l);
+      }
+      __syncthreads();
+      const float *x = a.x + (pr + r0) * a.vis + i0 + threadIdx.x;
+#pragma unroll 2
+      for (int row = 0; row < r1 - r0; row++, x += a.vis) {
+        const float st = stat[row];
+#pragma unroll
+        for (int k = 0; k < PT; k++)
+          if (i0 + k * kJoinThreads + (int)threadIdx.x < live) sum[k] += sm100::ex2(x[k * kJoinThreads] - st);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < PT; k++) {
+      const int i = i0 + k * kJoinThreads + threadIdx.x, j = token_of(u, i / kUnit) + i % kUnit;
+      if (i < live && j < u.n) a.wsum[((size_t)s * a.Hkv + kvh) * a.cap + j] += sum[k];
+    }
+  }
+}
+
+constexpr int kJoinSplits = 16;
+
+// Token splits. Few items: one wave of resident CTAs (444 slots, 8 items of 8192 units: 55 splits 58 us, 37 62 us, 74
+// 69 us). Many: about four waves, which even out ragged lengths, of 128 units a CTA or more (512 items of up to 1024
+// units: 4 splits 215 us, 2 235 us, 6 222 us). Never less than two units a warp.
+int choose_splits(const Attn4 &a, int ctas) {
+  const long long items = (long long)a.nseq * a.Hkv * a.tiles, units = a.vis / kUnit, slots = 148LL * ctas;
+  const long long s = slots / items >= 4 ? slots / items : std::min((4 * slots + items - 1) / items, units / 128);
+  return (int)std::max<long long>(1, std::min(s, units / (2 * kWarps)));
+}
+
+template <class E, int DK, bool WS>
+cudaError_t launch_attn_ws(const Attn4 &a, const E *q, E *out, cudaStream_t st, uint64_t *launches) {
+  auto kern = a.prow / a.tiles == kRows ? kv4_attn_kernel<E, DK, 1, WS> : kv4_attn_kernel<E, DK, 2, WS>;
+  cudaError_t e = smem_attr((const void *)kern, kAttnSmem<DK>);
+  if (e != cudaSuccess) return e;
+  kern<<<dim3(a.splits * a.tiles * a.Hkv, a.nseq), 32 * kWarps, kAttnSmem<DK>, st>>>(a, q, out);
+  *launches += 1;
+  e = cudaGetLastError();
+  if (e != cudaSuccess || (!WS && (a.splits == 1 || a.join))) return e;
+  const int rows = a.T * (a.H / a.Hkv);
+  const int joins = a.splits > 1 ? a.Hkv * rows : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(joins + (WS ? (a.vis + kSumTok - 1) / kSumTok * a.Hkv : 0), a.nseq);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  *launches += 1;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<E, DK, WS>, a, out, joins);
+}
 template <class E>
 cudaError_t launch_attn(const Attn4 &a, int dk, const E *q, E *out, cudaStream_t st, uint64_t *launches) {
-  const int rows = a.nseq * a.T * a.H;
-  const dim3 wg((a.max_len + 7) / 8, a.nseq * a.Hkv);
-  if (dk == 64) kv4_attn_kernel<E, 64><<<rows, 32, 0, st>>>(a, q, out);
-  else kv4_attn_kernel<E, 128><<<rows, 32, 0, st>>>(a, q, out);
-  *launches += 1;
-  if (a.wsum && a.max_len) {
-    if (dk == 64) kv4_wsum_kernel<E, 64><<<wg, 256, 0, st>>>(a, q);
-    else kv4_wsum_kernel<E, 128><<<wg, 256, 0, st>>>(a, q);
-    *launches += 1;
-  }
-  return cudaGetLastError();
+  if (dk == 64) return a.wsum ? launch_attn_ws<E, 64, true>(a, q, out, st, launches) : launch_attn_ws<E, 64, false>(a, q, out, st, launches);
+  return a.wsum ? launch_attn_ws<E, 128, true>(a, q, out, st, launches) : launch_attn_ws<E, 128, false>(a, q, out, st, launches);
 }
 
 }  // namespace
@@ -268,6 +977,14 @@ ORKB_ERR_WORD_SETTER(kv4_set_err_word)
 }  // namespace orkb
 
 using namespace orkb;
+
+// The context's split counters, at least n of them and zero (each launch leaves them so); nullptr without memory.
+static unsigned int *zeroed_counts(ork_npu *c, size_t n) {
+  const size_t had = c->capK;
+  if (!grow(&c->dK, &c->capK, n * sizeof(unsigned int))) return nullptr;
+  if (c->capK != had && cudaMemset(c->dK, 0, c->capK) != cudaSuccess) return nullptr;
+  return (unsigned int *)c->dK;
+}
 
 static int refuse(const char *name, const char *why) {
   fprintf(stderr, "[ork] ERROR %s: %s\n", name, why);
@@ -333,18 +1050,41 @@ int ork_b200_kv4_attn_async(ork_npu *c, const ork_b200_kv4 *kv, const ork_b200_k
   if (const char *why = cache_wrong(kv)) return refuse(name, why);
   if (a->type < ORK_B200_F32 || a->type > ORK_B200_BF16) return refuse(name, "unknown element type");
   if (a->H < 1 || a->H % kv->Hkv) return refuse(name, "H is a multiple of Hkv");
-  if (a->T < 1 || (long long)kv->nseq * a->T * a->H > 0x7fffffff) return refuse(name, "bad number of rows");
+  if (a->T < 1 || a->T > kv->cap || (long long)kv->nseq * a->T * a->H > 0x7fffffff) return refuse(name, "bad number of rows");
   if (a->q_ts < kv->dk || a->q_hs < kv->dk) return refuse(name, "a row stride below dk");
   if (a->max_len < 0 || a->max_len > kv->cap) return refuse(name, "max_len is 0 .. cap");
   if (a->window < 0 || a->sinks < 0) return refuse(name, "window and sinks are not negative");
   if (((uintptr_t)a->q | (uintptr_t)a->out) % elem_bytes(a->type)) return refuse(name, "rows are aligned to their type");
   DeviceGuard dg(c->device);
   if (!device_ptrs_ok(c, name, {kv->k, kv->v, kv->kp, kv->vp, a->q, a->out, a->len, a->wsum})) return -1;
-  Attn4 k = {kv->k, kv->v, (const __half *)kv->kp, (const __half *)kv->vp, kv->nseq, kv->Hkv, kv->cap, a->H, a->T,
-             a->window, a->sinks, a->max_len, a->q_ts, a->q_hs, a->len, a->scale, a->wsum, nullptr};
-  if (a->wsum && !grow(&c->dW, &c->capW, (size_t)kv->nseq * a->T * a->H * sizeof(float2)))
-    return refuse(name, "out of device memory");
-  k.stat = (float2 *)c->dW;
+  if (a->max_len == 0) {
+    const cudaError_t e = cudaMemsetAsync(a->out, 0, (size_t)kv->nseq * a->T * a->H * kv->dk * elem_bytes(a->type), c->stream);
+    if (e != cudaSuccess) log_err(name, e);
+    return e == cudaSuccess ? 0 : -1;
+  }
+  Attn4 k = {};
+  k.kc = kv->k, k.vc = kv->v, k.kp = (const __half *)kv->kp, k.vp = (const __half *)kv->vp;
+  k.nseq = kv->nseq, k.Hkv = kv->Hkv, k.cap = kv->cap, k.H = a->H, k.T = a->T;
+  k.window = a->window < a->max_len ? a->window : 0;  // a window over everything is none
+  k.sinks = std::min(a->sinks, a->max_len);
+  k.max_len = a->max_len, k.q_ts = a->q_ts, k.q_hs = a->q_hs, k.len = a->len, k.scale = a->scale, k.wsum = a->wsum;
+  const int rows = a->T * (a->H / kv->Hkv), tr = rows > kRows ? 2 * kRows : kRows;
+  k.tiles = (rows + tr - 1) / tr;
+  k.prow = k.tiles * tr;
+  // sinks and window, whole units of each
+  long long vis = (a->max_len + kUnit - 1) / kUnit * kUnit;
+  if (k.window) vis = std::min<long long>(vis, (long long)k.window + k.T + k.sinks + 3 * kUnit);
+  k.vis = (int)(vis / kUnit * kUnit);
+  k.splits = choose_splits(k, kv->dk == 128 && (tr > kRows || a->type == ORK_B200_F32) ? 2 : 3);
+  k.qvec = ((uintptr_t)a->q | (size_t)a->q_ts * elem_bytes(a->type) | (size_t)a->q_hs * elem_bytes(a->type)) % 16 == 0;
+  k.join = k.splits > 1 && k.splits <= kJoinSplits && !a->wsum;
+  const size_t prows = (size_t)k.nseq * k.Hkv * k.prow, mlb = (prows * k.splits * sizeof(float2) + 255) / 256 * 256;
+  const size_t pob = k.splits > 1 ? prows * k.splits * kv->dk * 4 : 0, xb = a->wsum ? prows * k.vis * 4 : 0;
+  if ((k.splits > 1 || a->wsum) && !grow(&c->dW, &c->capW, mlb + pob + xb)) return refuse(name, "out of device memory");
+  if (k.join && !(k.done = zeroed_counts(c, (size_t)k.nseq * k.Hkv * k.tiles))) return refuse(name, "out of device memory");
+  k.pml = (float2 *)c->dW;
+  k.po = (float *)((uint8_t *)c->dW + mlb);
+  k.x = (float *)((uint8_t *)c->dW + mlb + pob);
   const cudaError_t e = with_elem(a->type, [&](auto *t) {
     using E = std::remove_pointer_t<decltype(t)>;
     return launch_attn<E>(k, kv->dk, (const E *)a->q, (E *)a->out, c->stream, &c->launches);

@@ -28,6 +28,8 @@ struct ork_npu {
   size_t capX = 0;
   void *dW = nullptr;    // workspace of the long-context operators (kv4.cu, evict.cu)
   size_t capW = 0;
+  void *dK = nullptr;    // split counters of the 4-bit attention, zero between launches (kv4.cu)
+  size_t capK = 0;
   void *ltabs = nullptr; // device tables of persistent-layer pointer lists (layer.cu)
   void *dG = nullptr;    // 16 bytes, zero between calls: the argmax's running key and CTA count (decode_glue.cu)
   unsigned int *dF = nullptr;  // tensor-core split-K tile flags, orkb::kTcFlagTiles x 2 words, zero between launches
