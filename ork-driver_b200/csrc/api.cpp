@@ -122,6 +122,13 @@ bool grow(void **p, size_t *cap, size_t need) {
   return true;
 }
 
+unsigned int *zeroed_counts(ork_npu *c, size_t n) {
+  const size_t had = c->capK;
+  if (!grow(&c->dK, &c->capK, (kAttnCounts + n) * sizeof(unsigned int))) return nullptr;
+  if (c->capK != had && cudaMemsetAsync(c->dK, 0, c->capK, c->stream) != cudaSuccess) return nullptr;
+  return (unsigned int *)c->dK;
+}
+
 bool overlaps(const void *a, size_t an, const void *b, size_t bn) {
   const uintptr_t a0 = (uintptr_t)a, a1 = a0 + an, b0 = (uintptr_t)b, b1 = b0 + bn;
   return a0 < b1 && b0 < a1;

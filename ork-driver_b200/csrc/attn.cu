@@ -1,16 +1,17 @@
 // attn.cu -- attention of packed rows (prompts, or chunks after a cached prefix) with a sliding window and sink
 // keys (include/ork_b200.h: ork_b200_attn_async), on the 5th-generation tensor cores.
 //
-// A CTA owns two tiles of 128 query rows of one kv head and streams the keys that any of them sees, 128 at a time:
+// One CTA per SM takes items, two tiles of 128 query rows of one kv head, and streams the keys that any of them sees, 128
+// at a time; the loads and products of an item begin under the end of the one before:
 //   S = Q K^T     128 x 128 x dk, both operands in shared memory, S in tensor memory (fp32)
 //   P = 2^(S sc - m)  online softmax, a thread per row; P goes back to tensor memory in 16 bits, over S
 //   O += P V      128 x dk x 128, P from tensor memory, V in shared memory as it lies (N-major), O in tensor memory
 // The two tiles alternate: while one is in its softmax the tensor cores work for the other. A row of a tile is a
 // (token, head) pair, `pack` heads of the group (its largest power of two, at most 8) side by side, so that few tokens
 // still fill a tile, and the tile's tokens, whose windows end at different keys, are few.
-// Roles (320 threads): warps 0-3 and 4-7 the softmax and output of tile 0 and 1, warp 8 issues the products, warp 9
-// the TMA loads into a ring of 128 x dk slots that K and V tiles share. A row of S is read twice, for its maximum and
-// for its weights, 32 columns at a time: tensor memory has bandwidth to spare, and a whole row in registers spills.
+// Roles (three warpgroups): 0 and 1 the softmax and output of tile 0 and 1; of the third, warp 8 issues the products and
+// warp 9 the TMA loads into a ring of 128 x dk slots that K and V tiles share. It gives most of its registers to the
+// others, whose threads hold a row of S each.
 // The running maximum follows only when it rises by more than 2^8, so that O is seldom scaled; weights stay below 256.
 // Masks are applied to the tiles that hold an edge; tiles that no row sees are not visited.
 // A value of V that is not finite reaches rows that do not see it (0 * inf): a row whose result is not finite is
@@ -24,6 +25,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstdio>
+#include <type_traits>
 
 #include "elem.cuh"
 #include "errword.cuh"
@@ -49,7 +51,7 @@ __device__ __forceinline__ bool seq_of(const ork_b200_attn &a, int s, Seq *o) {
                   k1 <= a.k_rows && k1 - o->k0 <= a.max_k;
   o->tq = ok ? q1 - o->q0 : 0;
   o->tk = ok ? k1 - o->k0 : 0;
-  if (!ok && threadIdx.x == 0) {
+  if (!ok) {
     atomicOr(&g_attn_error, 1u);
     err_word_set();
   }
@@ -57,7 +59,7 @@ __device__ __forceinline__ bool seq_of(const ork_b200_attn &a, int s, Seq *o) {
 }
 
 constexpr int kTile = 128;    // query rows of a tile, keys of a step
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
 constexpr float kRise = 8.0f;  // log2 of the rise of a maximum that O is scaled for
 
 __device__ __forceinline__ void attn_failed() {
@@ -90,12 +92,20 @@ __device__ __forceinline__ uint32_t pack2(float x, float y, const __nv_bfloat16 
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if any is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Shared memory: the two Q tiles, the ring, 4 KB for each softmax warp's output, barriers, items.
 template <int DK>
 struct Smem {
-  static constexpr int kSlots = DK == 128 ? 5 : 8;
+  static constexpr int kSlots = DK == 128 ? 4 : 8;
   static constexpr int kTileBytes = kTile * DK * 2, kChunk = kTile * 128;  // a 64-column block of a tile
-  static constexpr int kBars = 1 + 2 * kSlots + 6;
-  static constexpr int kBytes = 1024 + (2 + kSlots) * kTileBytes + kBars * 8 + 16;
+  static constexpr int kStage = (2 + kSlots) * kTileBytes, kBar = kStage + 8 * 4096;
+  static constexpr int kBars = 2 + 2 * kSlots + 6 + 4, kItem = kBar + kBars * 8;
+  static constexpr int kBytes = 1024 + kItem + 2 * 80 + 16;
 };
 static_assert(Smem<128>::kBytes <= 232448 && Smem<64>::kBytes <= 232448, "shared memory");
 
@@ -117,7 +127,7 @@ __device__ __forceinline__ Steps steps_of(int p0, int p1, int window, int sinks)
 
 // One row from its visible keys alone, by a warp: lane l holds dims l + 32 u.
 template <class E, int DK>
-__device__ __noinline__ void slow_row(const ork_b200_attn &a, const Seq &s, int tok, int h) {
+__device__ __forceinline__ void slow_row(const ork_b200_attn &a, const Seq &s, int tok, int h) {
   constexpr int PER = DK / 32;
   const int lane = threadIdx.x & 31, kvh = h / (a.H / a.Hkv), p = s.tk - s.tq + tok;
   const E *q = (const E *)a.q + (s.q0 + tok) * a.q_ts + h * a.q_hs;
@@ -138,38 +148,54 @@ __device__ __noinline__ void slow_row(const ork_b200_attn &a, const Seq &s, int 
   for (int u = 0; u < PER; u++) out[lane + 32 * u] = from_f32<E>(l == 0.0f ? 0.0f : o[u] / l);
 }
 
+// An item: a head group of a sequence, and a pair of tiles of its tokens.
+struct Item {
+  Seq s;
+  int kvh, h0, tok0, back;  // first head and token; position of token 0
+  Steps st[2], all;         // of the tiles, of either
+  int end;                  // there are no more items
+};
+static_assert(sizeof(Item) <= 80, "an item's place");
+// Items are numbered by tile pair (the last ones first: they see most), then sequence, then head group. False: nothing
+// to do.
+__device__ __forceinline__ bool item_of(const ork_b200_attn &a, int it, int pairs, int lp, int groups, Item *o) {
+  const int hg = it % groups, sq = it / groups % a.nseq, pair = pairs - 1 - it / groups / a.nseq, per = kTile >> lp;
+  o->h0 = hg << lp, o->kvh = o->h0 / (a.H / a.Hkv), o->tok0 = pair * 2 * per;
+  if (!seq_of(a, sq, &o->s) || o->tok0 >= o->s.tq) return false;
+  o->back = o->s.tk - o->s.tq;
+#pragma unroll
+  for (int t = 0; t < 2; t++) {
+    const int t0 = o->tok0 + t * per, t1 = min(t0 + per, o->s.tq) - 1;
+    o->st[t] = steps_of(o->back + t0, t0 <= t1 ? o->back + t1 : -1, a.window, a.sinks);
+  }
+  o->all = steps_of(o->back + o->tok0, o->back + min(o->tok0 + 2 * per, o->s.tq) - 1, a.window, a.sinks);
+  o->end = 0;
+  return true;
+}
+
 template <class E, int DK>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_kernel(const ork_b200_attn a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                const __grid_constant__ CUtensorMap mv, int pack, int groups) {
+                const __grid_constant__ CUtensorMap mv, int lp, int groups, int pairs, int items, unsigned int *count) {
   using M = Smem<DK>;
   constexpr int SLOTS = M::kSlots, CH = DK / 64;
   extern __shared__ uint8_t raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-  const uint32_t sq = sm100::smem_addr(smem), sring = sq + 2 * M::kTileBytes, bars = sring + SLOTS * M::kTileBytes;
-  const uint32_t qfull = bars, full = bars + 8, empty = full + 8 * SLOTS, sfull = empty + 8 * SLOTS, pfull = sfull + 16,
-                 ofull = pfull + 16;
-  uint32_t *slot = (uint32_t *)(smem + (2 + SLOTS) * M::kTileBytes + M::kBars * 8);
+  const uint32_t sq = sm100::smem_addr(smem), sring = sq + 2 * M::kTileBytes, bars = sq + M::kBar;
+  const uint32_t qfull = bars, qempty = bars + 8, full = bars + 16, empty = full + 8 * SLOTS, sfull = empty + 8 * SLOTS,
+                 pfull = sfull + 16, ofull = pfull + 16, ifull = ofull + 16, iempty = ifull + 16;
+  Item *place = (Item *)(smem + M::kItem);  // [2]
+  uint32_t *slot = (uint32_t *)(smem + M::kItem + 2 * 80);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-
-  // the item: a head group of a sequence, and a pair of tiles of its tokens, the last ones first (they see most)
-  const int hg = blockIdx.x % groups, kvh = hg * pack / (a.H / a.Hkv), h0 = hg * pack;
-  const int per = kTile / pack, tok0 = (gridDim.x / groups - 1 - blockIdx.x / groups) * 2 * per;
-  Seq s;
-  if (!seq_of(a, blockIdx.y, &s) || tok0 >= s.tq) return;
-  const int back = s.tk - s.tq;  // position of token 0
-  Steps st[2], all;
-#pragma unroll
-  for (int t = 0; t < 2; t++) {
-    const int t0 = tok0 + t * per, t1 = min(t0 + per, s.tq) - 1;
-    st[t] = steps_of(back + t0, t0 <= t1 ? back + t1 : -1, a.window, a.sinks);
-  }
-  all = steps_of(back + tok0, back + min(tok0 + 2 * per, s.tq) - 1, a.window, a.sinks);
+  const int per = kTile >> lp;
 
   if (threadIdx.x == 0) {
-    sm100::bar_init(qfull, 1);
+    sm100::bar_init(qfull, 1), sm100::bar_init(qempty, 1);
     for (int i = 0; i < SLOTS; i++) sm100::bar_init(full + 8 * i, 1), sm100::bar_init(empty + 8 * i, 1);
-    for (int t = 0; t < 2; t++) sm100::bar_init(sfull + 8 * t, 1), sm100::bar_init(pfull + 8 * t, 4), sm100::bar_init(ofull + 8 * t, 1);
+    for (int t = 0; t < 2; t++) {
+      sm100::bar_init(sfull + 8 * t, 1), sm100::bar_init(pfull + 8 * t, 4);
+      sm100::bar_init(ofull + 8 * t, 1), sm100::bar_init(ifull + 8 * t, 1), sm100::bar_init(iempty + 8 * t, 9);
+    }
     sm100::bar_init_fence();
   }
   if (warp == 8) sm100::tmem_alloc(sm100::smem_addr(slot), 512);
@@ -177,209 +203,296 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *slot;
-  const int steps = all.count();
-
-  if (warp == 9) {  // ---- loads
-    if (lane == 0 && steps > 0) {
-      sm100::bar_expect(qfull, 2 * M::kTileBytes);
-      for (int t = 0; t < 2; t++)
-        for (int c = 0; c < CH; c++)
-          sm100::tma_load_3d(sq + t * M::kTileBytes + c * M::kChunk, &mq, 64 * c, h0, s.q0 + tok0 + t * per, qfull);
-      for (int i = 0; i < 2 * steps; i++) {  // K of step 0, V of step 0, K of step 1, ...
-        const int sl = i % SLOTS;
-        if (i >= SLOTS && !sm100::bar_wait(empty + 8 * sl, (i / SLOTS - 1) & 1)) {
-          attn_failed();
-          break;
-        }
-        sm100::bar_expect(full + 8 * sl, M::kTileBytes);
-        for (int c = 0; c < CH; c++)
-          sm100::tma_load_3d(sring + sl * M::kTileBytes + c * M::kChunk, i & 1 ? (const void *)&mv : (const void *)&mk, 64 * c, kvh,
-                             s.k0 + all.tile(i >> 1) * kTile, full + 8 * sl);
-      }
-    }
-  } else if (warp == 8) {  // ---- products
-    constexpr uint32_t ids = inst_desc<E>(kTile, false), ido = inst_desc<E>(DK, true);
-    bool ok = steps == 0 || sm100::bar_wait(qfull, 0);
-    int np[2] = {0, 0};  // P tiles consumed
-    // S of tile t at step i from the K in slot sl
-    auto score = [&](int t, int sl) {
-      const uint64_t qa = desc_k(sq + t * M::kTileBytes), kb = desc_k(sring + sl * M::kTileBytes);
-#pragma unroll
-      for (int c = 0; c < CH; c++)
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-          sm100::tc_mma(tmem + t * kTile, qa + (uint64_t)(c * (M::kChunk >> 4) + 2 * k), kb + (uint64_t)(c * (M::kChunk >> 4) + 2 * k),
-                        ids, c | k ? 1u : 0u);
-      sm100::tc_commit(sfull + 8 * t);
-    };
-    auto wait_full = [&](int i) { return sm100::bar_wait(full + 8 * (i % SLOTS), (i / SLOTS) & 1); };
-    if (steps > 0 && ok) {
-      ok = wait_full(0);
-      sm100::tc_fence_after();
-      if (ok && lane == 0) {
+  bool ok = true;
+  Item w;
+  // registers: 2 x 208 + 88 = 3 x 168, what the block was launched with
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 9 && lane == 0) {  // ---- items, and loads: Q, then K of step 0, V of step 0, K of step 1, ...
+      int nq = 0, g = 0, k = 0;    // Q pairs, ring tiles, items so far
+      for (int it = blockIdx.x; ok; it = (int)(gridDim.x + atomicAdd(count, 1u))) {
+        w.end = it >= items;
+        if (!w.end && !item_of(a, it, pairs, lp, groups, &w)) continue;
+        ok = k < 2 || sm100::bar_wait(iempty + 8 * (k & 1), ((k >> 1) - 1) & 1);
+        if (!ok) break;
+        place[k & 1] = w;
+        sm100::bar_arrive(ifull + 8 * (k & 1));
+        k++;
+        if (w.end) break;
+        if (w.all.count() == 0) continue;
+        ok = nq == 0 || sm100::bar_wait(qempty, (nq - 1) & 1);
+        if (!ok) break;
+        nq++;
+        sm100::bar_expect(qfull, 2 * M::kTileBytes);
         for (int t = 0; t < 2; t++)
-          if (st[t].has(all.tile(0))) score(t, 0);
-        sm100::tc_commit(empty);
-      }
-    }
-    for (int i = 0; i < steps && ok; i++) {
-      const int kt = all.tile(i), vi = 2 * i + 1, ki = 2 * i + 2;
-      ok = wait_full(vi) && (i + 1 == steps || wait_full(ki));
-      if (!ok) break;
-      const uint32_t sv = sring + vi % SLOTS * M::kTileBytes;
-      if (kt * kTile + kTile > s.tk) {  // rows past the sequence: zeros
-        for (int at = (s.tk - kt * kTile) * 8 + lane; at < kTile * 8; at += 32)
-#pragma unroll
           for (int c = 0; c < CH; c++)
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + c * M::kChunk + at * 16), "r"(0) : "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-      }
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
-        if (st[t].has(kt)) {
-          ok = ok && sm100::bar_wait(pfull + 8 * t, np[t] & 1);
+            sm100::tma_load_3d(sq + t * M::kTileBytes + c * M::kChunk, &mq, 64 * c, w.h0, w.s.q0 + w.tok0 + t * per, qfull);
+        for (int i = 0; i < 2 * w.all.count(); i++, g++) {
+          const int sl = g % SLOTS;
+          ok = g < SLOTS || sm100::bar_wait(empty + 8 * sl, (g / SLOTS - 1) & 1);
           if (!ok) break;
-          sm100::tc_fence_after();
-          if (lane == 0) {
-            const uint64_t vb = desc_mn(sv, M::kChunk);
-#pragma unroll
-            for (int k = 0; k < kTile / 16; k++)
-              sm100::tc_mma_ts(tmem + 256 + t * 128, tmem + t * kTile + 8 * k, vb + (uint64_t)(k * (2048 >> 4)), ido,
-                               np[t] || k ? 1u : 0u);
-          }
-          np[t]++;
+          sm100::bar_expect(full + 8 * sl, M::kTileBytes);
+          for (int c = 0; c < CH; c++)
+            sm100::tma_load_3d(sring + sl * M::kTileBytes + c * M::kChunk, i & 1 ? (const void *)&mv : (const void *)&mk, 64 * c,
+                               w.kvh, w.s.k0 + w.all.tile(i >> 1) * kTile, full + 8 * sl);
         }
-        if (lane == 0 && i + 1 < steps && st[t].has(all.tile(i + 1))) score(t, ki % SLOTS);
+      }
+      if (!ok) attn_failed();
+      // the last CTA to be done with the count leaves it zero for the next launch
+      __threadfence();
+      if (atomicInc(count + 1, gridDim.x - 1) == gridDim.x - 1) *count = 0;
+    } else if (warp == 8) {  // ---- products, issued by one elected lane from operands the whole warp agrees on
+      constexpr uint32_t ids = inst_desc<E>(kTile, false), ido = inst_desc<E>(DK, true);
+      constexpr uint32_t kSlot = M::kTileBytes >> 4;
+      const uint64_t qd = desc_k(sq), kd = desc_k(sring), vd = desc_mn(sring, M::kChunk);
+      int nq = 0, g = 0, np[2] = {0, 0};  // Q pairs, ring slot of the next K, P tiles so far
+      int gp = 0;                         // parity of the ring's round at g
+      auto wait_full = [&](int off) {     // ring tile g + off, off < SLOTS
+        const int sl = g + off < SLOTS ? g + off : g + off - SLOTS;
+        return sm100::bar_wait(full + 8 * sl, g + off < SLOTS ? gp : gp ^ 1);
+      };
+      auto slot_of = [&](int off) { return (uint32_t)(g + off < SLOTS ? g + off : g + off - SLOTS); };
+      // S of tile t from the K in slot sl
+      auto score = [&](int t, uint32_t sl) {
+        const uint64_t qa = qd + t * kSlot, kb = kd + sl * kSlot;
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            sm100::tc_mma(tmem + t * kTile, qa + (c * (M::kChunk >> 4) + 2 * k), kb + (c * (M::kChunk >> 4) + 2 * k), ids, c | k ? 1u : 0u);
+        sm100::tc_commit(sfull + 8 * t);
+      };
+      for (int k = 0; ok; k++) {
+        ok = sm100::bar_wait(ifull + 8 * (k & 1), (k >> 1) & 1);
+        if (!ok) break;
+        const Item *pl = place + (k & 1);
+        auto steps_at = [&](const Steps &x) { return Steps{sm100::uniform(x.ns), sm100::uniform(x.lo), sm100::uniform(x.hi)}; };
+        const Steps all = steps_at(pl->all), mine[2] = {steps_at(pl->st[0]), steps_at(pl->st[1])};
+        const int tk = sm100::uniform(pl->s.tk), end = sm100::uniform(pl->end);
+        if (lane == 0) sm100::bar_arrive(iempty + 8 * (k & 1));
+        if (end) break;
+        const int steps = all.count();
+        if (steps == 0) continue;
+        bool any[2] = {false, false};
+        ok = sm100::bar_wait(qfull, nq & 1) && wait_full(0);
+        if (!ok) break;
+        nq++;
+        sm100::tc_fence_after();
+        if (sm100::elect_one()) {
+#pragma unroll
+          for (int t = 0; t < 2; t++)
+            if (mine[t].has(all.tile(0))) score(t, (uint32_t)g);
+          sm100::tc_commit(empty + 8 * g);
+          if (steps == 1) sm100::tc_commit(qempty);
+        }
+        __syncwarp();
+        for (int i = 0; i < steps && ok; i++) {
+          const int kt = all.tile(i);
+          const bool more = i + 1 < steps;
+          const uint32_t vsl = slot_of(1), ksl = slot_of(2);
+          ok = wait_full(1) && (!more || wait_full(2));
+          if (!ok) break;
+          if (kt * kTile + kTile > tk) {  // rows past the sequence: zeros
+            const uint32_t sv = sring + vsl * M::kTileBytes;
+            for (int at = (tk - kt * kTile) * 8 + lane; at < kTile * 8; at += 32)
+#pragma unroll
+              for (int c = 0; c < CH; c++)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + c * M::kChunk + at * 16), "r"(0) : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+          const int next = more ? all.tile(i + 1) : 0;
+#pragma unroll
+          for (int t = 0; t < 2; t++) {
+            const bool now = mine[t].has(kt), then = more && mine[t].has(next);
+            if (now) {
+              ok = ok && sm100::bar_wait(pfull + 8 * t, np[t] & 1);
+              if (!ok) break;
+              np[t]++;
+              sm100::tc_fence_after();
+            }
+            if (sm100::elect_one()) {
+              if (now) {
+                const uint64_t vb = vd + vsl * kSlot;
+#pragma unroll
+                for (int e = 0; e < kTile / 16; e++)
+                  sm100::tc_mma_ts(tmem + 256 + t * 128, tmem + t * kTile + 8 * e, vb + e * (2048 >> 4), ido, any[t] || e ? 1u : 0u);
+              }
+              if (then) score(t, ksl);
+              if (t == 1) {
+                sm100::tc_commit(empty + 8 * vsl);
+                if (more) sm100::tc_commit(empty + 8 * ksl);
+                if (i + 2 == steps) sm100::tc_commit(qempty);
+              }
+            }
+            __syncwarp();
+            any[t] = any[t] || now;
+          }
+          g += 2;
+          if (g >= SLOTS) g -= SLOTS, gp ^= 1;
+        }
+        if (!ok) break;
+        if (sm100::elect_one()) {
+#pragma unroll
+          for (int t = 0; t < 2; t++)
+            if (any[t]) sm100::tc_commit(ofull + 8 * t);
+        }
         __syncwarp();
       }
-      if (ok && lane == 0) {
-        sm100::tc_commit(empty + 8 * (vi % SLOTS));
-        if (i + 1 < steps) sm100::tc_commit(empty + 8 * (ki % SLOTS));
-      }
-      __syncwarp();
+      if (!ok && lane == 0) attn_failed();
     }
-    if (!ok && lane == 0) attn_failed();
-    if (ok && lane == 0)
-      for (int t = 0; t < 2; t++)
-        if (np[t]) sm100::tc_commit(ofull + 8 * t);
-  } else if (warp < 8) {  // ---- softmax of tile t, a thread per row
-    const int t = warp >> 2, row = threadIdx.x & 127, tok = tok0 + t * per + row / pack, h = h0 + row % pack;
-    const int p = back + tok;
-    // positions of the warp's rows, of those that are rows of the sequence
-    const int w0 = back + tok0 + t * per + (warp & 3) * 32 / pack, w1 = back + tok0 + t * per + ((warp & 3) * 32 + 31) / pack;
-    const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * kTile, to = ts - t * kTile + 256 + t * 128;
+  } else {  // ---- softmax of tile t, a thread per row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = warp >> 2, row = threadIdx.x & 127, wrow = row & 96;
+    const uint32_t ts = tmem + ((uint32_t)wrow << 16) + t * kTile, to = ts - t * kTile + 256 + t * 128;
+    const uint32_t stage = sq + M::kStage + warp * 4096;
     const float sc = a.scale * 1.4426950408889634f;
-    float m = -INFINITY, l = 0.0f;
-    int n = 0;  // steps done
-    bool ok = true;
-    for (int i = 0; i < steps; i++) {
-      const int kt = all.tile(i), j0 = kt * kTile;
-      if (!st[t].has(kt)) continue;
-      ok = sm100::bar_wait(sfull + 8 * t, n & 1);
+    const float2 sc2 = make_float2(sc, sc);
+    int ns = 0, no = 0;  // steps and items with any so far
+    for (int k = 0; ok; k++) {
+      ok = sm100::bar_wait(ifull + 8 * (k & 1), (k >> 1) & 1);
       if (!ok) break;
-      sm100::tc_fence_after();
-      uint32_t x[2][32];
-      const bool edge = !(j0 + kTile - 1 <= w0 && (a.window == 0 || j0 > w1 - a.window || j0 + kTile <= a.sinks));
-      const int hi = p - j0, lo = a.window ? p - a.window - j0 : -1, sk = a.sinks - j0;
-      auto mask = [&](int c, uint32_t (&v)[32]) {
+      const Item *pl = place + (k & 1);
+      if (pl->end) break;
+      const int tok0 = pl->tok0 + t * per, p = pl->back + tok0 + (row >> lp);
+      // a tile of keys has no edge for the warp's rows if it begins at `inner` or before, and after `outer` or before the
+      // sinks' end
+      const int inner = pl->back + tok0 + (wrow >> lp) - kTile + 1, outer = pl->back + tok0 + ((wrow + 31) >> lp) - a.window;
+      const int first = ns, sinks = pl->st[t].ns, lo = pl->st[t].lo, last = pl->st[t].hi;
+      float m = -INFINITY, l = 0.0f;
+      for (int kt = sinks ? 0 : lo; kt <= last; kt = kt + 1 == sinks ? lo : kt + 1) {
+        const int j0 = kt * kTile;
+        ok = sm100::bar_wait(sfull + 8 * t, ns & 1);
+        if (!ok) break;
+        sm100::tc_fence_after();
+        const bool edge = !(j0 <= inner && (a.window == 0 || j0 > outer || j0 + kTile <= a.sinks));
+        uint32_t x[4][32];
+        float mx[4];
+        auto load = [&](int c) { sm100::tmem_ld32(ts + 32 * c, x[c]); };
+        auto mask_max = [&](int c) {
+          if (edge) {  // the row's visible columns as bits: up to its position, after the window's begin or among the sinks
+            auto below = [&](int n) { return n <= 32 * c ? 0u : n >= 32 * c + 32 ? 0xffffffffu : (1u << (n - 32 * c)) - 1u; };
+            const uint32_t see = below(p - j0 + 1) & (~below(a.window ? p - a.window - j0 + 1 : 0) | below(a.sinks - j0));
 #pragma unroll
-        for (int e = 0; e < 32; e++) {
-          const int j = 32 * c + e;
-          if (!(j <= hi && (j > lo || j < sk))) v[e] = 0xff800000u;
-        }
-      };
-      float mx[4];
-      sm100::tmem_ld32(ts, x[0]);
+            for (int e = 0; e < 32; e++)
+              if (!(see >> e & 1u)) x[c][e] = 0xff800000u;
+          }
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        sm100::tmem_ld_wait(x[c & 1]);
-        if (c < 3) sm100::tmem_ld32(ts + 32 * c + 32, x[(c + 1) & 1]);
-        else sm100::tmem_ld32(ts, x[0]);
-        if (edge) mask(c, x[c & 1]);
-        mx[c] = __uint_as_float(x[c & 1][0]);
+          for (int q = 0; q < 4; q++) {
+            auto f = [&](int e) { return __uint_as_float(x[c][e + q]); };
+            mx[q] = max3(c ? mx[q] : f(0), f(0), f(4));
+            mx[q] = max3(mx[q], f(8), f(12));
+            mx[q] = max3(mx[q], f(16), f(20));
+            mx[q] = max3(mx[q], f(24), f(28));
+          }
+        };
+        float2 sum = make_float2(0.0f, 0.0f);
+        auto weights = [&](int c, float2 mu) {
+          uint32_t pk[16];
+          float2 part = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int e = 1; e < 32; e++) mx[c] = fmaxf(mx[c], __uint_as_float(x[c & 1][e]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      const bool rise = (top - m) * sc > kRise;
-      if (__any_sync(0xffffffffu, rise)) {
-        const float k = rise ? sm100::ex2((m - top) * sc) : 1.0f;
-        if (rise) m = top;
-        l *= k;
-        if (n) {
+          for (int e = 0; e < 16; e++) {
+            float2 v = sm100::fma2(make_float2(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), sc2, mu);
+            v = make_float2(sm100::ex2(v.x), sm100::ex2(v.y));
+            if (e & 1) part = sm100::add2(part, v);
+            else sum = sm100::add2(sum, v);
+            pk[e] = pack2(v.x, v.y, (const E *)nullptr);
+          }
+          sum = sm100::add2(sum, part);
+          sm100::tmem_st16(ts + 16 * c, pk);
+        };
+        load(0), load(1);
+        sm100::tmem_ld_wait(x[0]), sm100::tmem_ld_wait(x[1]);
+        load(2), load(3);
+        mask_max(0), mask_max(1);
+        sm100::tmem_ld_wait(x[2]), sm100::tmem_ld_wait(x[3]);
+        mask_max(2), mask_max(3);
+        const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+        if (!(top < INFINITY)) l = __int_as_float(0x7fc00000);  // an infinity or a NaN among the logits: see slow_row
+        const bool rise = (top - m) * sc > kRise;
+        if (__any_sync(0xffffffffu, rise)) {
+          const float k2 = rise ? sm100::ex2((m - top) * sc) : 1.0f;
+          if (rise) m = top;
+          l *= k2;
+          if (ns > first) {
+#pragma unroll 1
+            for (int c = 0; c < DK / 32; c++) {
+              uint32_t o[32];
+              sm100::tmem_ld32(to + 32 * c, o);
+              sm100::tmem_ld_wait(o);
 #pragma unroll
-          for (int c = 0; c < DK / 32; c++) {
-            uint32_t o[32];
-            sm100::tmem_ld32(to + 32 * c, o);
-            sm100::tmem_ld_wait(o);
-#pragma unroll
-            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * k);
-            sm100::tmem_st32(to + 32 * c, o);
+              for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * k2);
+              sm100::tmem_st32(to + 32 * c, o);
+            }
           }
         }
-      }
-      const float2 sc2 = make_float2(sc, sc), mu = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-m * sc, -m * sc);
-      float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        const float2 mu = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-m * sc, -m * sc);
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        uint32_t pk[16];
-        sm100::tmem_ld_wait(x[c & 1]);
-        if (c < 3) sm100::tmem_ld32(ts + 32 * c + 32, x[(c + 1) & 1]);
-        if (edge) mask(c, x[c & 1]);
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          float2 v = sm100::fma2(make_float2(__uint_as_float(x[c & 1][2 * e]), __uint_as_float(x[c & 1][2 * e + 1])), sc2, mu);
-          v = make_float2(sm100::ex2(v.x), sm100::ex2(v.y));
-          sum[e & 1] = sm100::add2(sum[e & 1], v);
-          pk[e] = pack2(v.x, v.y, (const E *)nullptr);
-        }
-        sm100::tmem_st16(ts + 16 * c, pk);
+        for (int c = 0; c < 4; c++) weights(c, mu);
+        l += sum.x + sum.y;
+        sm100::tmem_st_wait();
+        sm100::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) sm100::bar_arrive(pfull + 8 * t);
+        ns++;
       }
-      sum[0] = sm100::add2(sum[0], sum[1]);
-      l += sum[0].x + sum[0].y;
-      sm100::tmem_st_wait();
-      sm100::tc_fence_before();
+      if (!ok) break;
+      if (ns > first) {
+        ok = sm100::bar_wait(ofull + 8 * t, no & 1);
+        if (!ok) break;
+        no++;
+        sm100::tc_fence_after();
+      }
+      // rows of 64 columns through shared memory, so that a store writes whole 128-byte lines
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      bool fin = true;
+      const Seq seq = pl->s;
+      const int h0 = pl->h0;
       __syncwarp();
-      if (lane == 0) sm100::bar_arrive(pfull + 8 * t);
-      n++;
-    }
-    if (n && ok) {
-      ok = sm100::bar_wait(ofull + 8 * t, 0);
-      sm100::tc_fence_after();
+      if (lane == 0) sm100::bar_arrive(iempty + 8 * (k & 1));
+      E *const base = (E *)a.out + (long long)seq.q0 * a.o_ts + 8 * (lane & 7);
+#pragma unroll 1
+      for (int c = 0; c < CH; c++) {
+#pragma unroll 1
+        for (int hf = 0; hf < 2; hf++) {
+          uint32_t o[32];
+          if (ns > first) {
+            sm100::tmem_ld32(to + 64 * c + 32 * hf, o);
+            sm100::tmem_ld_wait(o);
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e++) {
+            const float v = ns > first ? __uint_as_float(o[e]) * inv : 0.0f;
+            fin = fin && fabsf(v) <= 3.402823466e38f;
+            o[e] = __float_as_uint(v);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            auto two = [&](int q) { return pack2(__uint_as_float(o[8 * e + q]), __uint_as_float(o[8 * e + q + 1]), base); };
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + (((4 * hf + e) ^ (lane & 7)) << 4)),
+                         "r"(two(0)), "r"(two(2)), "r"(two(4)), "r"(two(6))
+                         : "memory");
+          }
+        }
+        __syncwarp();
+#pragma unroll 2
+        for (int j = 0; j < 8; j++) {
+          const int rr = 4 * j + (lane >> 3), tk = tok0 + ((wrow + rr) >> lp), h = h0 + ((wrow + rr) & ((1 << lp) - 1));
+          uint4 v;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)));
+          if (tk < seq.tq) *reinterpret_cast<uint4 *>(base + (long long)tk * a.o_ts + (long long)h * a.o_hs + 64 * c) = v;
+        }
+        __syncwarp();
+      }
+      const int tok = tok0 + (row >> lp), h = h0 + (row & ((1 << lp) - 1));
+      for (unsigned bad = __ballot_sync(0xffffffffu, tok < seq.tq && !fin); bad; bad &= bad - 1) {
+        const int from = __ffs(bad) - 1;
+        slow_row<E, DK>(a, seq, __shfl_sync(0xffffffffu, tok, from), __shfl_sync(0xffffffffu, h, from));
+      }
     }
     if (!ok && lane == 0) attn_failed();
-    const bool live = tok < s.tq && ok;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    E *out = (E *)a.out + (long long)(s.q0 + tok) * a.o_ts + (long long)h * a.o_hs;
-    bool fin = true;
-#pragma unroll
-    for (int c = 0; c < DK / 32; c++) {
-      uint32_t o[32];
-      if (n) {
-        sm100::tmem_ld32(to + 32 * c, o);
-        sm100::tmem_ld_wait(o);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; e++) o[e] = 0;
-      }
-#pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-          v[k] = l == 0.0f ? 0.0f : __uint_as_float(o[e + k]) * inv;
-          fin = fin && fabsf(v[k]) <= 3.402823466e38f;
-        }
-        if (live)
-          *reinterpret_cast<uint4 *>(out + 32 * c + e) =
-              make_uint4(pack2(v[0], v[1], out), pack2(v[2], v[3], out), pack2(v[4], v[5], out), pack2(v[6], v[7], out));
-      }
-    }
-    for (unsigned bad = __ballot_sync(0xffffffffu, live && !fin); bad; bad &= bad - 1) {
-      const int from = __ffs(bad) - 1;
-      slow_row<E, DK>(a, s, __shfl_sync(0xffffffffu, tok, from), __shfl_sync(0xffffffffu, h, from));
-    }
   }
   sm100::tc_fence_before();
   __syncthreads();
@@ -409,7 +522,7 @@ bool make_map(CUtensorMap *m, const ork_b200_attn &a, const void *p, int heads, 
 }
 
 template <class E, int DK>
-cudaError_t launch_attn(const ork_b200_attn &a, cudaStream_t st) {
+cudaError_t launch_attn(const ork_b200_attn &a, unsigned int *count, cudaStream_t st) {
   const int G = a.H / a.Hkv, pack = std::min(G & -G, 8), per = kTile / pack, groups = a.H / pack;
   CUtensorMap mq, mk, mv;
   if (!encoder() || !make_map(&mq, a, a.q, a.H, a.q_rows, a.q_ts, a.q_hs, pack, per)) return cudaErrorInvalidValue;
@@ -420,8 +533,10 @@ cudaError_t launch_attn(const ork_b200_attn &a, cudaStream_t st) {
   const int smem = Smem<DK>::kBytes;
   const cudaError_t e = smem_attr((const void *)attn_kernel<E, DK>, smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)((a.max_q + 2 * per - 1) / (2 * per) * groups), a.nseq);
-  attn_kernel<E, DK><<<grid, kThreads, smem, st>>>(a, mq, mk, mv, pack, groups);
+  const int pairs = (a.max_q + 2 * per - 1) / (2 * per);
+  const long long items = (long long)pairs * groups * a.nseq;
+  if (items > 0x7fffff00) return cudaErrorInvalidValue;
+  attn_kernel<E, DK><<<(int)std::min<long long>(items, 148), kThreads, smem, st>>>(a, mq, mk, mv, __builtin_ctz(pack), groups, pairs, (int)items, count);
   return cudaGetLastError();
 }
 
@@ -468,9 +583,12 @@ extern "C" int ork_b200_attn_async(ork_npu *c, const ork_b200_attn *a) {
   ork_b200_attn d = *a;
   d.window = d.window < d.max_k ? d.window : 0;  // a window over everything is none
   d.sinks = std::min(d.sinks, d.max_k);
-  const cudaError_t e = d.type == ORK_B200_F16
-                            ? (d.dk == 64 ? launch_attn<__half, 64>(d, c->stream) : launch_attn<__half, 128>(d, c->stream))
-                            : (d.dk == 64 ? launch_attn<__nv_bfloat16, 64>(d, c->stream) : launch_attn<__nv_bfloat16, 128>(d, c->stream));
+  unsigned int *count = zeroed_counts(c, 0);
+  if (!count) return refuse("out of device memory");
+  const bool f16 = d.type == ORK_B200_F16, wide = d.dk == 128;
+  const cudaError_t e = f16 ? (wide ? launch_attn<__half, 128>(d, count, c->stream) : launch_attn<__half, 64>(d, count, c->stream))
+                            : (wide ? launch_attn<__nv_bfloat16, 128>(d, count, c->stream)
+                                    : launch_attn<__nv_bfloat16, 64>(d, count, c->stream));
   c->launches += 1;
   if (e != cudaSuccess) {
     log_err("ork_b200_attn_async", e);

@@ -978,14 +978,6 @@ ORKB_ERR_WORD_SETTER(kv4_set_err_word)
 
 using namespace orkb;
 
-// The context's split counters, at least n of them and zero (each launch leaves them so); nullptr without memory.
-static unsigned int *zeroed_counts(ork_npu *c, size_t n) {
-  const size_t had = c->capK;
-  if (!grow(&c->dK, &c->capK, n * sizeof(unsigned int))) return nullptr;
-  if (c->capK != had && cudaMemset(c->dK, 0, c->capK) != cudaSuccess) return nullptr;
-  return (unsigned int *)c->dK;
-}
-
 static int refuse(const char *name, const char *why) {
   fprintf(stderr, "[ork] ERROR %s: %s\n", name, why);
   return -1;
@@ -1081,7 +1073,11 @@ int ork_b200_kv4_attn_async(ork_npu *c, const ork_b200_kv4 *kv, const ork_b200_k
   const size_t prows = (size_t)k.nseq * k.Hkv * k.prow, mlb = (prows * k.splits * sizeof(float2) + 255) / 256 * 256;
   const size_t pob = k.splits > 1 ? prows * k.splits * kv->dk * 4 : 0, xb = a->wsum ? prows * k.vis * 4 : 0;
   if ((k.splits > 1 || a->wsum) && !grow(&c->dW, &c->capW, mlb + pob + xb)) return refuse(name, "out of device memory");
-  if (k.join && !(k.done = zeroed_counts(c, (size_t)k.nseq * k.Hkv * k.tiles))) return refuse(name, "out of device memory");
+  if (k.join) {
+    unsigned int *z = zeroed_counts(c, (size_t)k.nseq * k.Hkv * k.tiles);
+    if (!z) return refuse(name, "out of device memory");
+    k.done = z + kAttnCounts;
+  }
   k.pml = (float2 *)c->dW;
   k.po = (float *)((uint8_t *)c->dW + mlb);
   k.x = (float *)((uint8_t *)c->dW + mlb + pob);

@@ -28,7 +28,7 @@ struct ork_npu {
   size_t capX = 0;
   void *dW = nullptr;    // workspace of the long-context operators (kv4.cu, evict.cu)
   size_t capW = 0;
-  void *dK = nullptr;    // split counters of the 4-bit attention, zero between launches (kv4.cu)
+  void *dK = nullptr;    // counters of the long-context operators, zero between launches (zeroed_counts)
   size_t capK = 0;
   void *ltabs = nullptr; // device tables of persistent-layer pointer lists (layer.cu)
   void *dG = nullptr;    // 16 bytes, zero between calls: the argmax's running key and CTA count (decode_glue.cu)
@@ -87,6 +87,10 @@ bool device_ptrs_ok(const ork_npu *c, const char *name, std::initializer_list<co
 // on the context is refused meanwhile (message + true), the reference's one-job-in-flight contract
 // (include/ork/chain.h:126-133) made a checked error.
 bool async_in_flight(const ork_npu *c, const char *name);
+// Device counters that are zero, and that every launch leaves zero: kAttnCounts for attn.cu, then n for kv4.cu;
+// nullptr without memory.
+constexpr size_t kAttnCounts = 4;
+unsigned int *zeroed_counts(ork_npu *c, size_t n);
 bool overlaps(const void *a, size_t an, const void *b, size_t bn);
 // Enqueues one decode layer on device pointers (layer.cu); W = {q, k, v, o, gate, up, down}.
 int layer_enqueue(ork_npu *c, const struct ork_layer_dims *d, ork_w *const *W, const float *attn_norm,

@@ -41,6 +41,15 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
   return true;
 }
 
+// one lane of a converged warp, known to the compiler as one
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+// the first lane's value, known to be the same for the whole warp
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // bytes (a multiple of 16, both addresses 16-byte aligned) from global to shared memory, completing on bar
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
