@@ -205,9 +205,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *slot;
   bool ok = true;
   Item w;
-  // registers: 2 x 208 + 88 = 3 x 168, what the block was launched with
+  // registers: 2 x 216 + 72 = 3 x 168, what the block was launched with
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 9 && lane == 0) {  // ---- items, and loads: Q, then K of step 0, V of step 0, K of step 1, ...
       int nq = 0, g = 0, k = 0;    // Q pairs, ring tiles, items so far
       for (int it = blockIdx.x; ok; it = (int)(gridDim.x + atomicAdd(count, 1u))) {
@@ -342,8 +342,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok && lane == 0) attn_failed();
     }
   } else {  // ---- softmax of tile t, a thread per row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int t = warp >> 2, row = threadIdx.x & 127, wrow = row & 96;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int t = warp >> 2, wrow = (warp & 3) * 32, row = wrow + lane;
     const uint32_t ts = tmem + ((uint32_t)wrow << 16) + t * kTile, to = ts - t * kTile + 256 + t * 128;
     const uint32_t stage = sq + M::kStage + warp * 4096;
     const float sc = a.scale * 1.4426950408889634f;
@@ -353,12 +353,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = sm100::bar_wait(ifull + 8 * (k & 1), (k >> 1) & 1);
       if (!ok) break;
       const Item *pl = place + (k & 1);
-      if (pl->end) break;
-      const int tok0 = pl->tok0 + t * per, p = pl->back + tok0 + (row >> lp);
+      if (sm100::uniform(pl->end)) break;
+      const int tok0 = sm100::uniform(pl->tok0) + t * per, pos0 = sm100::uniform(pl->back) + tok0, p = pos0 + (row >> lp);
       // a tile of keys has no edge for the warp's rows if it begins at `inner` or before, and after `outer` or before the
       // sinks' end
-      const int inner = pl->back + tok0 + (wrow >> lp) - kTile + 1, outer = pl->back + tok0 + ((wrow + 31) >> lp) - a.window;
-      const int first = ns, sinks = pl->st[t].ns, lo = pl->st[t].lo, last = pl->st[t].hi;
+      const int inner = pos0 + (wrow >> lp) - kTile + 1, outer = pos0 + ((wrow + 31) >> lp) - a.window;
+      const int first = ns, sinks = sm100::uniform(pl->st[t].ns), lo = sm100::uniform(pl->st[t].lo), last = sm100::uniform(pl->st[t].hi);
       float m = -INFINITY, l = 0.0f;
       for (int kt = sinks ? 0 : lo; kt <= last; kt = kt + 1 == sinks ? lo : kt + 1) {
         const int j0 = kt * kTile;
@@ -446,8 +446,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // rows of 64 columns through shared memory, so that a store writes whole 128-byte lines
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       bool fin = true;
-      const Seq seq = pl->s;
-      const int h0 = pl->h0;
+      const Seq seq = {sm100::uniform(pl->s.q0), sm100::uniform(pl->s.tq), sm100::uniform(pl->s.k0), sm100::uniform(pl->s.tk)};
+      const int h0 = sm100::uniform(pl->h0);
       __syncwarp();
       if (lane == 0) sm100::bar_arrive(iempty + 8 * (k & 1));
       E *const base = (E *)a.out + (long long)seq.q0 * a.o_ts + 8 * (lane & 7);
