@@ -212,7 +212,7 @@ int ork_b200_kv4_attn_async(ork_npu *ctx, const ork_b200_kv4 *c, const ork_b200_
 /* Eviction from a cache by accumulated attention weight. Of the n = len[s] tokens of each sequence and kv head,
  * min(n, keep) are kept: the first `sinks`, the last `recent`, then those with the largest score [nseq][Hkv][cap]
  * (ties: the lowest slot; a NaN counts as minus infinity); sinks + recent <= keep. The kept rows move, in their
- * order, from each of `nplanes` source planes src[i] [nseq][Hkv][cap] rows of row_bytes[i] (a multiple of 4) to
+ * order, from each of `nplanes` source planes src[i] [nseq][Hkv][cap] rows of row_bytes[i] (a multiple of 4, at most 65536) to
  * slots 0.. of dst[i] [nseq][Hkv][dcap], dcap >= keep: the planes of a 4-bit cache, or of an fp32 one. No source
  * overlaps a destination. kept [nseq][Hkv][keep]: the source slots (-1 past the kept ones); score_out
  * [nseq][Hkv][dcap]: their scores (0 up to `keep`), ready to accumulate on; len_out [nseq]: min(n, keep).

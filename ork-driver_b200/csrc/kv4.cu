@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstdio>
+#include <type_traits>
 
 #include "elem.cuh"
 #include "errword.cuh"
@@ -24,19 +25,25 @@ namespace {
 
 constexpr int kGroup = 64;  // dims that share a step and a lowest value
 
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+
 __device__ __forceinline__ void kv4_error() {
   atomicOr(&g_kv4_error, 1u);
   err_word_set();
 }
 
 // ---- rows into the cache and back ------------------------------------------------------------------------------
-// A thread handles 8 consecutive dims of k or of v of one row and head: one 32-bit word of codes, so that a
-// group's 8 threads find its lowest and largest value with three shuffles and a row's words are stored (loaded)
-// by consecutive threads. Blocks stride over (row, head, k or v) items of a sequence (blockIdx.y).
+// A thread handles 8 consecutive dims of k or of v of one row and head, one 32-bit word of codes: a group's 8 threads
+// find its lowest and largest value with three shuffles, and dk / 4 threads read and write a token's k and v of a head
+// whole. A warp keeps its heads and steps through the rows of its sequence (blockIdx.y).
+// The division by the step, which has to be the IEEE one for the codes to be the definition's, is a product with the
+// step's reciprocal wherever that is sure to round to the same code, and is done again where it is not (a quotient within
+// 1e-5 of the middle between two codes; the product is off by 6e-6 at most).
+// Bound by memory: the store of 49145 rows of 8 heads of 128 bf16 dims reads 201 MB and writes 57 MB (100 us, the load back 50 us; issue slots 65 % used).
 constexpr int kRowThreads = 256;
 
 struct Rows {
-  int nseq, Hkv, dk, cap, rows;
+  int nseq, Hkv, cap, rows;
   long long ts, hs;
   const int *start, *pos;
 };
@@ -94,66 +101,120 @@ __device__ __forceinline__ void store8(E *p, bool vec, const float (&x)[8]) {
   }
 }
 
-template <class E, bool STORE>
+__device__ __forceinline__ float min_nan(float a, float b, float c) {  // NaN if any is
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+template <class E, int DK, bool STORE, bool VEC>
 __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(Rows r, E *k, E *v, uint32_t *kc, uint32_t *vc,
-                                                               __half2 *kp, __half2 *vp, bool vec) {
-  const int s = blockIdx.y, words = r.dk / 8, lane = threadIdx.x & 31;
+                                                               __half2 *kp, __half2 *vp) {
+  constexpr int WORDS = DK / 8, LANES = 2 * WORDS;  // words of a row; threads of a (row, head): k's, then v's
+  const int s = blockIdx.y, lane = threadIdx.x & 31;
   const int row0 = r.start ? r.start[s] : s * r.rows;
   const int n = r.start ? r.start[s + 1] - row0 : r.rows;
   const int slot0 = r.pos ? r.pos[s] : 0;
-  const long long items = (long long)(n > 0 ? n : 0) * r.Hkv * 2 * words;  // a multiple of 8: groups stay whole
-  for (long long at = (long long)blockIdx.x * kRowThreads + threadIdx.x; at < items;
-       at += (long long)gridDim.x * kRowThreads) {
-    const int w = (int)(at % words);
-    const long long rh = at / words;
-    const bool is_v = rh & 1;
-    const int h = (int)((rh >> 1) % r.Hkv), t = (int)((rh >> 1) / r.Hkv);
-    const long long slot = (long long)slot0 + t;
-    if (slot < 0 || slot >= r.cap) {  // the same for a group's eight threads
-      kv4_error();
-      continue;
+  // teams of LANES threads: team i takes head i % Hkv and every `step`-th row from i / Hkv on
+  const int teams = gridDim.x * (kRowThreads / LANES), step = teams / r.Hkv;
+  const int team = (blockIdx.x * kRowThreads + threadIdx.x) / LANES, h = team % r.Hkv, t0 = team / r.Hkv;
+  const int at = threadIdx.x % LANES, w = at % WORDS;
+  const bool is_v = at >= WORDS;
+  if (t0 >= step) return;  // whole teams; a group's threads stay together
+  // the rows whose slots the cache has
+  const long long first = slot0 < 0 ? -(long long)slot0 : 0, end = (long long)r.cap - slot0;
+  const int last = (int)max(0LL, min((long long)n, end));
+  if (at == 0 && (t0 < min((long long)n, first) || n > last)) kv4_error();
+  int t = t0;
+  if (t < first) t += (int)((min(first, (long long)n) - t + step - 1) / step) * step;
+  const long long hop = (long long)step * r.ts;
+  E *row = (is_v ? v : k) + ((long long)row0 + t) * r.ts + (long long)h * r.hs + 8 * w;
+  const size_t tok = ((size_t)s * r.Hkv + h) * r.cap + (size_t)((long long)slot0 + t);
+  uint32_t *code = (is_v ? vc : kc) + tok * WORDS + w;
+  __half2 *par = (is_v ? vp : kp) + tok * (DK / kGroup) + w / 8;
+  const unsigned mask = 0xffu << (lane & 24);
+  float next[8];
+  if constexpr (!STORE) {  // four rows at a time on their way: a row is little to ask for
+    for (; t < last; t += 4 * step, row += 4 * hop, code += 4 * step * WORDS, par += 4 * step * (DK / kGroup)) {
+      uint32_t c[4];
+      __half2 p[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+        if (t + u * step < last) c[u] = code[(long long)u * step * WORDS], p[u] = par[(long long)u * step * (DK / kGroup)];
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+        if (t + u * step < last) {
+          const float2 f = __half22float2(p[u]);
+          float x[8];
+          // code * step is exact in fp32: one rounding either way
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[i] = fmaf(__uint_as_float(0x4b000000u | ((c[u] >> (4 * i)) & 15u)) - 8388608.0f, f.x, f.y);
+          store8<E>(row + u * hop, VEC, x);
+        }
     }
-    E *row = (is_v ? v : k) + ((long long)row0 + t) * r.ts + (long long)h * r.hs + 8 * w;
-    const size_t tok = ((size_t)s * r.Hkv + h) * r.cap + (size_t)slot;
-    uint32_t *code = (is_v ? vc : kc) + tok * words + w;
-    __half2 *par = (is_v ? vp : kp) + tok * (r.dk / kGroup) + w / 8;
+    return;
+  }
+  if (STORE && t < last) load8<E>(row, VEC, next);
+  for (; t < last; t += step, row += hop, code += step * WORDS, par += step * (DK / kGroup)) {
     float x[8];
     if constexpr (STORE) {
-      load8<E>(row, vec, x);
-      float lo = x[0], hi = x[0];
-      bool fin = true;
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-        fin = fin && fabsf(x[i]) <= 3.402823466e38f;
-      }
-      const unsigned mask = 0xffu << (lane & 24);
+      for (int i = 0; i < 8; i++) x[i] = next[i];
+      if (t + step < last) load8<E>(row + hop, VEC, next);
+      float lo = min_nan(min_nan(x[0], x[1], x[2]), min_nan(x[3], x[4], x[5]), min_nan(x[6], x[7], x[7]));
+      float hi = max_nan(max_nan(x[0], x[1], x[2]), max_nan(x[3], x[4], x[5]), max_nan(x[6], x[7], x[7]));
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+        const float l2 = __shfl_xor_sync(mask, lo, o), h2 = __shfl_xor_sync(mask, hi, o);
+        lo = min_nan(lo, l2, l2);
+        hi = max_nan(hi, h2, h2);
       }
-      fin = __all_sync(mask, fin);
       // every operation rounds on its own, so that any IEEE implementation of the formulas gives these bits
-      __half step = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 65504.0f));
+      __half step2 = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 65504.0f));
       __half low = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
-      if (!fin) step = low = __ushort_as_half((unsigned short)0x7fff);
-      const float sf = __half2float(step), lf = __half2float(low);
-      uint32_t c = 0;
-      if (sf > 0.0f) {
+      if (!(fabsf(lo) <= 3.402823466e38f && fabsf(hi) <= 3.402823466e38f)) step2 = low = __ushort_as_half((unsigned short)0x7fff);
+      const float sf = __half2float(step2), lf = __half2float(low);
+      uint32_t c;
+      {
+        using namespace sm100;
+        float inv = 0.0f;  // no step, no codes
+        if (sf > 0.0f) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf * 15.0f));
+        const float2 two23 = both(8388608.0f);
+        float off = 0.0f, r4[8];
+        float2 m[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-          c |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], lf), sf)), 0.0f), 15.0f) << (4 * i);
+        for (int i = 0; i < 4; i++) {
+          // the quotient over 15 clamped to [0, 1]; m: the code plus 2^23, rounded to an integer by that addition
+          const float2 d = add2(make_float2(x[2 * i], x[2 * i + 1]), both(-lf));
+          const float2 q = make_float2(__saturatef(d.x * inv), __saturatef(d.y * inv));
+          m[i] = fma2(q, both(15.0f), two23);
+          const float2 z = add2(m[i], both(-8388608.0f));
+          const float2 e = fma2(q, both(15.0f), mul2(z, both(-1.0f)));
+          off = fmaxf(off, fmaxf(fabsf(e.x), fabsf(e.y)));
+          r4[2 * i] = z.x, r4[2 * i + 1] = z.y;
+        }
+        // four codes side by side in the low bits of 2^23 + c0 + 16 c1 + 256 c2 + 4096 c3
+        const float a = fmaf(r4[3], 4096.0f, fmaf(r4[2], 256.0f, fmaf(r4[1], 16.0f, m[0].x)));
+        const float b = fmaf(r4[7], 4096.0f, fmaf(r4[6], 256.0f, fmaf(r4[5], 16.0f, m[2].x)));
+        c = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x5410);
+        if (off > 0.49999f) {
+          c = 0;
+#pragma unroll 1
+          for (int i = 0; i < 8; i++) {
+            float y = x[0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) y = i == j ? x[j] : y;
+            c |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(y, lf), sf)), 0.0f), 15.0f) << (4 * i);
+          }
+        }
       }
       *code = c;
-      if ((w & 7) == 0) *par = __halves2half2(step, low);
-    } else {
-      const uint32_t c = *code;
-      const float2 p = __half22float2(*par);
-#pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = __fadd_rn(__fmul_rn((float)((c >> (4 * i)) & 15u), p.x), p.y);
-      store8<E>(row, vec, x);
+      if ((w & 7) == 0) *par = __halves2half2(step2, low);
     }
   }
 }
@@ -279,7 +340,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // an 8 x 8 tile o
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 // x as fp16 pairs: the rounded values, and what they leave
 __device__ __forceinline__ void split2(float2 x, uint32_t &hi, uint32_t &lo) {
   const __half2 h = __float22half2_rn(x);
@@ -1005,15 +1065,22 @@ static int kv4_rows(ork_npu *c, const ork_b200_kv4 *kv, const void *k, const voi
   if (!device_ptrs_ok(c, name, {kv->k, kv->v, kv->kp, kv->vp, k, v, start, pos})) return -1;
   if (rows == 0) return 0;
   const bool vec = ((uintptr_t)k | (uintptr_t)v | (size_t)ts * es | (size_t)hs * es) % 16 == 0;
-  const Rows r = {kv->nseq, kv->Hkv, kv->dk, kv->cap, rows, ts, hs, start, pos};
-  const long long items = (long long)rows * kv->Hkv * 2 * (kv->dk / 8);
-  const long long most = std::max<long long>(1, 148LL * 8 / kv->nseq);
-  const dim3 grid((unsigned)std::min<long long>((items + kRowThreads - 1) / kRowThreads, most), kv->nseq);
+  const Rows r = {kv->nseq, kv->Hkv, kv->cap, rows, ts, hs, start, pos};
+  // teams of a (row, head): a multiple of Hkv, so that every thread has a head; about 8 blocks an SM
+  const long long per = kRowThreads / (kv->dk / 4), want = ((long long)rows * kv->Hkv + per - 1) / per;
+  const long long most = std::max<long long>(148LL * 8 / kv->nseq, (kv->Hkv + per - 1) / per);
+  const dim3 grid((unsigned)std::min(want, most), kv->nseq);
   const cudaError_t e = with_elem(type, [&](auto *t) {
     using E = std::remove_pointer_t<decltype(t)>;
-    auto kern = store ? kv4_rows_kernel<E, true> : kv4_rows_kernel<E, false>;
-    kern<<<grid, kRowThreads, 0, c->stream>>>(r, (E *)k, (E *)v, (uint32_t *)kv->k, (uint32_t *)kv->v, (__half2 *)kv->kp,
-                                              (__half2 *)kv->vp, vec);
+    auto go = [&](auto aligned) {
+      constexpr bool V = decltype(aligned)::value;
+      auto kern = kv->dk == 64 ? (store ? kv4_rows_kernel<E, 64, true, V> : kv4_rows_kernel<E, 64, false, V>)
+                               : (store ? kv4_rows_kernel<E, 128, true, V> : kv4_rows_kernel<E, 128, false, V>);
+      kern<<<grid, kRowThreads, 0, c->stream>>>(r, (E *)k, (E *)v, (uint32_t *)kv->k, (uint32_t *)kv->v, (__half2 *)kv->kp,
+                                                (__half2 *)kv->vp);
+    };
+    if (vec) go(std::true_type());
+    else go(std::false_type());
     return cudaGetLastError();
   });
   c->launches += 1;
