@@ -278,6 +278,7 @@ struct Attn4 {
   int vis;            // most tokens that a row range can see, a multiple of kUnit (x's row stride)
   float *po;          // partial outputs [nseq][Hkv][prow][splits][dk], normalised by nothing
   float2 *pml;        // their maxima (log2 units) and sums [nseq][Hkv][prow][splits]
+  float *stat;        // m + log2(sum) of every row [nseq][Hkv][prow], for wsum
   float *x;           // logits in log2 units [nseq][Hkv][prow][vis], kept for wsum
 };
 
@@ -380,11 +381,17 @@ struct Wide {
 };
 template <int DK>
 constexpr int kStages = DK == 128 ? 2 : 4;
-// CTAs that an SM holds: with both halves of fp32 queries, or two column tiles, the registers of three would spill
+// CTAs that an SM holds: with both halves of p * step, or two column tiles, the registers of three would spill
 template <class E, int DK, int NT>
 constexpr int kCtas = DK == 128 && (NT == 2 || sizeof(E) == 4) ? 2 : 3;
-template <int DK>
-constexpr int kAttnSmem = kWarps * (kStages<DK> * ((int)sizeof(Stage<DK>) + 8) + (int)sizeof(Wide<DK>));
+// q of a CTA: its bytes in the order the first product takes them, and the scales and sums of its rows
+template <int DK, int NT>
+struct Query {
+  uint4 d[NT][3][DK / kGroup][32];
+  float f[NT * kRows], sum[DK / kGroup][NT * kRows];
+};
+template <int DK, int NT>
+constexpr int kAttnSmem = kWarps * (kStages<DK> * ((int)sizeof(Stage<DK>) + 8) + (int)sizeof(Wide<DK>)) + (int)sizeof(Query<DK, NT>);
 
 template <int N>
 __device__ __forceinline__ void load_pars(const float *p, float (&x)[N]) {
@@ -439,7 +446,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   const int s = blockIdx.y, G = a.H / a.Hkv, rows = a.T * G;
   Stage<DK> *ring = reinterpret_cast<Stage<DK> *>(smem) + warp * NST;
   Wide<DK> *wide = reinterpret_cast<Wide<DK> *>(smem + kWarps * NST * sizeof(Stage<DK>)) + warp;
-  const uint32_t bars = sm100::smem_addr(smem + kWarps * (NST * sizeof(Stage<DK>) + sizeof(Wide<DK>))) + warp * NST * 8;
+  Query<DK, NT> *qm = reinterpret_cast<Query<DK, NT> *>(smem + kWarps * (NST * sizeof(Stage<DK>) + sizeof(Wide<DK>)));
+  const uint32_t bars = sm100::smem_addr(qm + 1) + warp * NST * 8;
   if (lane < NST) sm100::bar_init(bars + 8 * lane, 1);
   sm100::bar_init_fence();
   __syncwarp();
@@ -460,12 +468,9 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
       next += cnt;
     }
 
-  // q of row r of each tile: byte 2 - d of the integers of the lane's words i, even dims then odd ones
-  uint32_t qd[NT][3][NG][2][2];
-  float fs[NT][2], qs[NT][NG][2];  // of the rows 2 c and 2 c + 1 that the accumulators hold
-#pragma unroll
-  for (int y = 0; y < NT; y++) {
-    const int row = tile * TR + y * kRows + r;
+  // q of row r of tile y, by warp y: byte 2 - d of the integers of the lane's words, even dims then odd ones
+  if (warp < NT) {
+    const int y = warp, row = tile * TR + y * kRows + r;
     const bool live = row < rows;
     const E *qr = q + ((long long)s * a.T + row / G) * a.q_ts + (long long)(kvh * G + row % G) * a.q_hs;
     float x[NG][16], mx = 0.0f;
@@ -488,7 +493,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
     fin = (__ballot_sync(0xffffffffu, fin) & quad) == quad;
     const int e = fin ? max(-100, min(100, 146 - (int)(__float_as_uint(mx) >> 23))) : 0;
     const float up = pow2(e), f = fin ? a.scale * 1.4426950408889634f * pow2(-e) : __int_as_float(0x7fc00000);
-    float sums[NG];
+    if (c == 0) qm->f[y * kRows + r] = f;
 #pragma unroll
     for (int g = 0; g < NG; g++) {
       int w[16], sum = 0;
@@ -498,25 +503,30 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
         sum += w[i];
         w[i] += 0x808080;  // bytes of 128 + digit
       }
-      sums[g] = quad_sum((float)sum) * f;
+      const float total = quad_sum((float)sum) * f;
+      if (c == 0) qm->sum[g][y * kRows + r] = total;
 #pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int odd = 0; odd < 2; odd++) {
-          const int w4[4] = {w[8 * i + odd], w[8 * i + 2 + odd], w[8 * i + 4 + odd], w[8 * i + 6 + odd]};
-#pragma unroll
-          for (int d = 0; d < 3; d++) qd[y][d][g][i][odd] = bytes_of(w4, 2 - d) ^ 0x80808080u;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int from = (2 * c + i) * 4;
-      fs[y][i] = __shfl_sync(0xffffffffu, f, from);
-#pragma unroll
-      for (int g = 0; g < NG; g++) qs[y][g][i] = __shfl_sync(0xffffffffu, sums[g], from);
+      for (int d = 0; d < 3; d++) {
+        auto digit = [&](int i) {
+          const int w4[4] = {w[i], w[i + 2], w[i + 4], w[i + 6]};
+          return bytes_of(w4, 2 - d) ^ 0x80808080u;
+        };
+        qm->d[y][d][g][lane] = make_uint4(digit(0), digit(1), digit(8), digit(9));
+      }
     }
   }
+  __syncthreads();
+  float fs[NT][2], qs[NT][NG][2];  // of the rows 2 c and 2 c + 1 that the accumulators hold
+#pragma unroll
+  for (int y = 0; y < NT; y++)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      fs[y][i] = qm->f[y * kRows + 2 * c + i];
+#pragma unroll
+      for (int g = 0; g < NG; g++) qs[y][g][i] = qm->sum[g][y * kRows + 2 * c + i];
+    }
 
+  const uint32_t qaddr = sm100::smem_addr(&qm->d[0][0][0][lane]);
   float o[NT][NG][4][4], z[NT][NG][2], l[NT][2], mrow[NT][2];
 #pragma unroll
   for (int y = 0; y < NT; y++)
@@ -617,13 +627,17 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
         for (int y = 0; y < NT; y++)
 #pragma unroll
           for (int d = 0; d < 3; d++) {
-            if (d == 0) mma_i80(acc[y][g], af[0], qd[y][d][g][0][0], qd[y][d][g][0][1]);
+            uint32_t qb[4];  // kept in shared memory, the registers are full
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(qb[0]), "=r"(qb[1]), "=r"(qb[2]), "=r"(qb[3])
+                         : "r"(qaddr + (uint32_t)(((y * 3 + d) * NG + g) * 512)));
+            if (d == 0) mma_i80(acc[y][g], af[0], qb[0], qb[1]);
             else {
 #pragma unroll
               for (int i = 0; i < 4; i++) acc[y][g][i] <<= 8;
-              mma_i8(acc[y][g], af[0], qd[y][d][g][0][0], qd[y][d][g][0][1]);
+              mma_i8(acc[y][g], af[0], qb[0], qb[1]);
             }
-            mma_i8(acc[y][g], af[1], qd[y][d][g][1][0], qd[y][d][g][1][1]);
+            mma_i8(acc[y][g], af[1], qb[2], qb[3]);
           }
       }
 #pragma unroll
@@ -817,6 +831,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
     }
   __syncthreads();
   constexpr int PER = 8;  // consecutive dims of one row
+  auto write_row = [&](int row, int d0, float m, float sum, const float (&v)[PER]) {
+    E *dst = out + (((long long)s * a.T + row / G) * a.H + kvh * G + row % G) * DK + d0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) dst[i] = from_f32<E>(sum == 0.0f ? 0.0f : v[i] / sum);
+    if (WS && d0 == 0) a.stat[((size_t)s * a.Hkv + kvh) * a.prow + row] = m == -INFINITY ? sum : m + log2f(sum);
+  };
   for (int at = threadIdx.x; at < TR * DK / PER; at += 32 * kWarps) {
     const int rr = at * PER / DK, d0 = at * PER % DK, row = tile * TR + rr;
     if (row >= rows) break;
@@ -833,15 +853,13 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
         for (int i = 0; i < PER; i++) v[i] = fmaf(k, so[(w * TR + rr) * LDO + d0 + i], v[i]);
     }
     const size_t pr = (((size_t)s * a.Hkv + kvh) * a.prow + row) * a.splits + split;
-    if ((WS || a.splits > 1) && d0 == 0) a.pml[pr] = make_float2(m, sum);
+    if (a.splits > 1 && d0 == 0) a.pml[pr] = make_float2(m, sum);
     if (a.splits > 1) {
       float4 *dst = reinterpret_cast<float4 *>(a.po + pr * DK + d0);
       dst[0] = make_float4(v[0], v[1], v[2], v[3]);
       dst[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-      E *dst = out + (((long long)s * a.T + row / G) * a.H + kvh * G + row % G) * DK + d0;
-#pragma unroll
-      for (int i = 0; i < PER; i++) dst[i] = from_f32<E>(sum == 0.0f ? 0.0f : v[i] / sum);
+      write_row(row, d0, m, sum, v);
     }
   }
   if (!a.join) return;
@@ -871,148 +889,154 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
         v[4] = fmaf(k, p1.x, v[4]), v[5] = fmaf(k, p1.y, v[5]), v[6] = fmaf(k, p1.z, v[6]), v[7] = fmaf(k, p1.w, v[7]);
       }
     }
-    E *dst = out + (((long long)s * a.T + row / G) * a.H + kvh * G + row % G) * DK + d0;
-#pragma unroll
-    for (int i = 0; i < PER; i++) dst[i] = from_f32<E>(sum == 0.0f ? 0.0f : v[i] / sum);
+    write_row(row, d0, m, sum, v);
   }
 }
 
-// Joins the splits of one row (the first `joins` blocks of x) and adds to wsum (the others, kSumTok tokens of one kv
-// head each): wsum[j] += sum over the rows of 2^(x_j - m) / l.
+// Joins the splits of one row, a CTA each.
 constexpr int kJoinThreads = 128;
-constexpr int kSumTok = 8 * kJoinThreads;
-template <class E, int DK, bool WS>
-__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Attn4 a, E *__restrict__ out, int joins) {
+template <class E, int DK>
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Attn4 a, E *__restrict__ out) {
   constexpr int NW = kJoinThreads / 32, PER = DK / 32;
   __shared__ float2 sml[NW];
   __shared__ float so[NW][DK];
   sm100::dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.H / a.Hkv, rows = a.T * G, s = blockIdx.y;
-  if ((int)blockIdx.x < joins) {
-    const int kvh = blockIdx.x / rows, row = blockIdx.x % rows;
-    const size_t pr = (((size_t)s * a.Hkv + kvh) * a.prow + row) * a.splits;
-    float m = -INFINITY, l = 0.0f, v[PER] = {};
-    for (int i0 = 32 * warp; i0 < a.splits; i0 += 32 * NW) {  // lane i: split i0 + i
-      const float2 ml = i0 + lane < a.splits ? a.pml[pr + i0 + lane] : make_float2(-INFINITY, 0.0f);
-      float mn = ml.x;
-      for (int off = 16; off; off >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
-      mn = fmaxf(mn, m);
-      const float was = m == mn ? 1.0f : sm100::ex2(m - mn);
-      const float k = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : sm100::ex2(ml.x - mn);
-      m = mn;
-      l = fmaf(k, ml.y, l * was);
+  const int kvh = blockIdx.x / rows, row = blockIdx.x % rows;
+  const size_t pr = (((size_t)s * a.Hkv + kvh) * a.prow + row) * a.splits;
+  float m = -INFINITY, l = 0.0f, v[PER] = {};
+  const int i0 = a.splits * warp / NW, i1 = a.splits * (warp + 1) / NW;  // the warp's splits, 32 at a time
+  for (int i = i0; i < i1; i += 32) {
+    const float2 ml = i + lane < i1 ? a.pml[pr + i + lane] : make_float2(-INFINITY, 0.0f);
+    float mn = ml.x;
+    for (int off = 16; off; off >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+    mn = fmaxf(mn, m);
+    const float was = m == mn ? 1.0f : sm100::ex2(m - mn);
+    const float k = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : sm100::ex2(ml.x - mn);
+    m = mn;
+    l = fmaf(k, ml.y, l * was);
 #pragma unroll
-      for (int d = 0; d < PER; d++) v[d] *= was;
-      const int cnt = min(32, a.splits - i0);
+    for (int d = 0; d < PER; d++) v[d] *= was;
+    const int cnt = min(32, i1 - i);
 #pragma unroll 16
-      for (int i = 0; i < cnt; i++) {
-        const float ki = __shfl_sync(0xffffffffu, k, i);
-        const float *po = a.po + (pr + i0 + i) * DK + PER * lane;
+    for (int j = 0; j < cnt; j++) {
+      const float kj = __shfl_sync(0xffffffffu, k, j);
+      const float *po = a.po + (pr + i + j) * DK + PER * lane;
 #pragma unroll
-        for (int d = 0; d < PER; d++) {
-          const float x = po[d];
-          if (ki != 0.0f) v[d] = fmaf(ki, x, v[d]);
-        }
+      for (int d = 0; d < PER; d++) {
+        const float x = po[d];
+        if (kj != 0.0f) v[d] = fmaf(kj, x, v[d]);
       }
-    }
-    for (int off = 16; off; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-    if (lane == 0) sml[warp] = make_float2(m, l);
-#pragma unroll
-    for (int d = 0; d < PER; d++) so[warp][PER * lane + d] = v[d];
-    __syncthreads();
-    if ((int)threadIdx.x < DK) {
-      float mm = -INFINITY, sum = 0.0f, x = 0.0f;
-#pragma unroll
-      for (int w = 0; w < NW; w++) mm = fmaxf(mm, sml[w].x);
-#pragma unroll
-      for (int w = 0; w < NW; w++) {
-        const float k = sml[w].x == -INFINITY && sml[w].y == 0.0f ? 0.0f : sm100::ex2(sml[w].x - mm);
-        sum = fmaf(k, sml[w].y, sum);
-        if (k != 0.0f) x = fmaf(k, so[w][threadIdx.x], x);
-      }
-      out[(((long long)s * a.T + row / G) * a.H + kvh * G + row % G) * DK + threadIdx.x] = from_f32<E>(sum == 0.0f ? 0.0f : x / sum);
-    }
-    return;
-  }
-  if constexpr (WS) {
-    constexpr int CH = 512, PT = kSumTok / kJoinThreads;  // rows at a time, tokens a thread
-    __shared__ float stat[CH];                            // m + log2 l
-    const int per = (a.vis + kSumTok - 1) / kSumTok, at = blockIdx.x - joins, kvh = at / per;
-    const Units u = units_of(a, seq_len(a, s));
-    const int i0 = at % per * kSumTok, live = u.all * kUnit;
-    if (i0 >= live) return;
-    const size_t pr = ((size_t)s * a.Hkv + kvh) * a.prow;
-    float sum[PT] = {};
-    for (int r0 = 0; r0 < rows; r0 += CH) {
-      const int r1 = min(rows, r0 + CH);
-      if (r0) __syncthreads();
-      for (int row = r0 + warp; row < r1; row += NW) {
-        const float2 *ml = a.pml + (pr + row) * a.splits;
-        float m = -INFINITY, l = 0.0f;
-        for (int i = lane; i < a.splits; i += 32) {
-          const float2 x = ml[i];
-          const float mn = fmaxf(m, x.x);
-          if (x.x != -INFINITY || x.y != 0.0f) l = fmaf(sm100::ex2(x.x - mn), x.y, m == mn ? l : l * sm100::ex2(m - mn));
-          m = mn;
-        }
-        for (int off = 16; off; off >>= 1) {
-          const float mo = __shfl_xor_sync(0xffffffffu, m, off), lo = __shfl_xor_sync(0xffffffffu, l, off), mn = fmaxf(m, mo);
-          l = (m == mn ? l : l * sm100::ex2(m - mn)) + (mo == mn ? lo : lo * sm100::ex2(mo - mn));
-          m = mn;
-        }
-        if (lane == 0) stat[row - r0] = m == -INFINITY ? (l == 0.0f ? 0.0f : l) : m + log2f(l);
-      }
-      __syncthreads();
-      const float *x = a.x + (pr + r0) * a.vis + i0 + threadIdx.x;
-#pragma unroll 2
-      for (int row = 0; row < r1 - r0; row++, x += a.vis) {
-        const float st = stat[row];
-#pragma unroll
-        for (int k = 0; k < PT; k++)
-          if (i0 + k * kJoinThreads + (int)threadIdx.x < live) sum[k] += sm100::ex2(x[k * kJoinThreads] - st);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < PT; k++) {
-      const int i = i0 + k * kJoinThreads + threadIdx.x, j = token_of(u, i / kUnit) + i % kUnit;
-      if (i < live && j < u.n) a.wsum[((size_t)s * a.Hkv + kvh) * a.cap + j] += sum[k];
     }
   }
+  for (int off = 16; off; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+  if (lane == 0) sml[warp] = make_float2(m, l);
+#pragma unroll
+  for (int d = 0; d < PER; d++) so[warp][PER * lane + d] = v[d];
+  __syncthreads();
+  sm100::dependents_launch();
+  if ((int)threadIdx.x >= DK) return;
+  float mm = -INFINITY, sum = 0.0f, x = 0.0f;
+#pragma unroll
+  for (int w = 0; w < NW; w++) mm = fmaxf(mm, sml[w].x);
+#pragma unroll
+  for (int w = 0; w < NW; w++) {
+    const float k = sml[w].x == -INFINITY && sml[w].y == 0.0f ? 0.0f : sm100::ex2(sml[w].x - mm);
+    sum = fmaf(k, sml[w].y, sum);
+    if (k != 0.0f) x = fmaf(k, so[w][threadIdx.x], x);
+  }
+  out[(((long long)s * a.T + row / G) * a.H + kvh * G + row % G) * DK + threadIdx.x] = from_f32<E>(sum == 0.0f ? 0.0f : x / sum);
+  if (a.wsum && threadIdx.x == 0) a.stat[((size_t)s * a.Hkv + kvh) * a.prow + row] = mm == -INFINITY ? sum : mm + log2f(sum);
 }
 
+// wsum[j] += sum over the rows of 2^(x_j - stat), four tokens a thread.
+constexpr int kSumThreads = 128, kSumTok = 4 * kSumThreads;
+__global__ void __launch_bounds__(kSumThreads) kv4_wsum_kernel(const Attn4 a) {
+  constexpr int CH = 256;  // rows at a time
+  __shared__ float stat[CH];
+  sm100::dependency_wait();
+  const int kvh = blockIdx.x % a.Hkv, s = blockIdx.y, rows = a.T * (a.H / a.Hkv);
+  const Units u = units_of(a, seq_len(a, s));
+  const int i0 = blockIdx.x / a.Hkv * kSumTok, live = u.all * kUnit, i = i0 + 4 * threadIdx.x;
+  if (i0 >= live) return;
+  const size_t pr = ((size_t)s * a.Hkv + kvh) * a.prow;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int r0 = 0; r0 < rows; r0 += CH) {
+    const int r1 = min(rows, r0 + CH);
+    if (r0) __syncthreads();
+    for (int row = r0 + threadIdx.x; row < r1; row += kSumThreads) stat[row - r0] = a.stat[pr + row];
+    __syncthreads();
+    if (i < live) {
+      const float *x = a.x + (pr + r0) * a.vis + i;
+#pragma unroll 8
+      for (int row = 0; row < r1 - r0; row++) {
+        const float4 v = __ldcs(reinterpret_cast<const float4 *>(x + (size_t)row * a.vis));
+        const float st = stat[row];  // a place that is not visible holds -inf
+        if (st != st) {              // a row that sees a NaN: so are its weights, of what it sees
+          auto add = [&](float &t, float y) { if (y != -INFINITY) t = st; };
+          add(sum.x, v.x), add(sum.y, v.y), add(sum.z, v.z), add(sum.w, v.w);
+          continue;
+        }
+        sum.x += sm100::ex2(v.x - st), sum.y += sm100::ex2(v.y - st);
+        sum.z += sm100::ex2(v.z - st), sum.w += sm100::ex2(v.w - st);
+      }
+    }
+  }
+  if (i >= live) return;
+  const int j = token_of(u, i / kUnit) + i % kUnit;
+  float *w = a.wsum + ((size_t)s * a.Hkv + kvh) * a.cap + j;
+  if (j < u.n) w[0] += sum.x;
+  if (j + 1 < u.n) w[1] += sum.y;
+  if (j + 2 < u.n) w[2] += sum.z;
+  if (j + 3 < u.n) w[3] += sum.w;
+}
+
+// Up to this many splits are joined by the last CTA of an item, in the launch itself; more by a CTA a row.
 constexpr int kJoinSplits = 16;
 
-// Token splits. Few items: one wave of resident CTAs (444 slots, 8 items of 8192 units: 55 splits 58 us, 37 62 us, 74
-// 69 us). Many: about four waves, which even out ragged lengths, of 128 units a CTA or more (512 items of up to 1024
-// units: 4 splits 215 us, 2 235 us, 6 222 us). Never less than two units a warp.
+// Token splits: the fewest waves of resident CTAs times what one takes, its units and about 45 units' worth (9 us) of
+// setting up and joining, fitted to 440 items of 1024 units in one wave (215 us) to four (242 us), 296 items (3 splits,
+// two waves, 159 us; 1 split 171 us, 6 splits 176 us) and 8 items of 8192 units (55 splits 58 us, 37 62 us, 74 69 us).
+// Two units a warp at least.
 int choose_splits(const Attn4 &a, int ctas) {
   const long long items = (long long)a.nseq * a.Hkv * a.tiles, units = a.vis / kUnit, slots = 148LL * ctas;
-  const long long s = slots / items >= 4 ? slots / items : std::min((4 * slots + items - 1) / items, units / 128);
-  return (int)std::max<long long>(1, std::min(s, units / (2 * kWarps)));
+  long long best = 1, least = 0;
+  for (long long s = 1; s == 1 || (s <= units / (2 * kWarps) && s <= 128); s++) {
+    const long long cost = (items * s + slots - 1) / slots * ((units + s - 1) / s + 45);
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  return (int)best;
 }
 
 template <class E, int DK, bool WS>
 cudaError_t launch_attn_ws(const Attn4 &a, const E *q, E *out, cudaStream_t st, uint64_t *launches) {
   auto kern = a.prow / a.tiles == kRows ? kv4_attn_kernel<E, DK, 1, WS> : kv4_attn_kernel<E, DK, 2, WS>;
-  cudaError_t e = smem_attr((const void *)kern, kAttnSmem<DK>);
+  const int smem = a.prow / a.tiles == kRows ? kAttnSmem<DK, 1> : kAttnSmem<DK, 2>;
+  cudaError_t e = smem_attr((const void *)kern, smem);
   if (e != cudaSuccess) return e;
-  kern<<<dim3(a.splits * a.tiles * a.Hkv, a.nseq), 32 * kWarps, kAttnSmem<DK>, st>>>(a, q, out);
+  kern<<<dim3(a.splits * a.tiles * a.Hkv, a.nseq), 32 * kWarps, smem, st>>>(a, q, out);
   *launches += 1;
   e = cudaGetLastError();
-  if (e != cudaSuccess || (!WS && (a.splits == 1 || a.join))) return e;
-  const int rows = a.T * (a.H / a.Hkv);
-  const int joins = a.splits > 1 ? a.Hkv * rows : 0;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(joins + (WS ? (a.vis + kSumTok - 1) / kSumTok * a.Hkv : 0), a.nseq);
-  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  *launches += 1;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<E, DK, WS>, a, out, joins);
+  if (e == cudaSuccess && a.splits > 1 && !a.join) {
+    cfg.gridDim = dim3(a.Hkv * a.T * (a.H / a.Hkv), a.nseq);
+    cfg.blockDim = dim3(kJoinThreads);
+    *launches += 1;
+    e = cudaLaunchKernelEx(&cfg, kv4_join_kernel<E, DK>, a, out);
+  }
+  if (e == cudaSuccess && WS) {
+    cfg.gridDim = dim3((a.vis + kSumTok - 1) / kSumTok * a.Hkv, a.nseq);
+    cfg.blockDim = dim3(kSumThreads);
+    *launches += 1;
+    e = cudaLaunchKernelEx(&cfg, kv4_wsum_kernel, a);
+  }
+  return e;
 }
 template <class E>
 cudaError_t launch_attn(const Attn4 &a, int dk, const E *q, E *out, cudaStream_t st, uint64_t *launches) {
@@ -1136,18 +1160,19 @@ int ork_b200_kv4_attn_async(ork_npu *c, const ork_b200_kv4 *kv, const ork_b200_k
   k.vis = (int)(vis / kUnit * kUnit);
   k.splits = choose_splits(k, kv->dk == 128 && (tr > kRows || a->type == ORK_B200_F32) ? 2 : 3);
   k.qvec = ((uintptr_t)a->q | (size_t)a->q_ts * elem_bytes(a->type) | (size_t)a->q_hs * elem_bytes(a->type)) % 16 == 0;
-  k.join = k.splits > 1 && k.splits <= kJoinSplits && !a->wsum;
-  const size_t prows = (size_t)k.nseq * k.Hkv * k.prow, mlb = (prows * k.splits * sizeof(float2) + 255) / 256 * 256;
-  const size_t pob = k.splits > 1 ? prows * k.splits * kv->dk * 4 : 0, xb = a->wsum ? prows * k.vis * 4 : 0;
-  if ((k.splits > 1 || a->wsum) && !grow(&c->dW, &c->capW, mlb + pob + xb)) return refuse(name, "out of device memory");
+  k.join = k.splits > 1 && k.splits <= kJoinSplits;
+  auto whole = [](size_t b) { return (b + 255) / 256 * 256; };
+  const size_t prows = (size_t)k.nseq * k.Hkv * k.prow, parts = k.splits > 1 ? prows * k.splits : 0;
+  const size_t mlb = whole(parts * sizeof(float2)), pob = whole(parts * kv->dk * 4), stb = a->wsum ? whole(prows * 4) : 0;
+  const size_t need = mlb + pob + stb + (a->wsum ? prows * k.vis * 4 : 0);
+  if (need && !grow(&c->dW, &c->capW, need)) return refuse(name, "out of device memory");
   if (k.join) {
     unsigned int *z = zeroed_counts(c, (size_t)k.nseq * k.Hkv * k.tiles);
     if (!z) return refuse(name, "out of device memory");
     k.done = z + kAttnCounts;
   }
-  k.pml = (float2 *)c->dW;
-  k.po = (float *)((uint8_t *)c->dW + mlb);
-  k.x = (float *)((uint8_t *)c->dW + mlb + pob);
+  uint8_t *ws = (uint8_t *)c->dW;
+  k.pml = (float2 *)ws, k.po = (float *)(ws + mlb), k.stat = (float *)(ws + mlb + pob), k.x = (float *)(ws + mlb + pob + stb);
   const cudaError_t e = with_elem(a->type, [&](auto *t) {
     using E = std::remove_pointer_t<decltype(t)>;
     return launch_attn<E>(k, kv->dk, (const E *)a->q, (E *)a->out, c->stream, &c->launches);
