@@ -189,6 +189,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int per = kTile >> lp;
 
+  if (warp == 9 && lane < 3)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &mq : lane == 1 ? &mk : &mv) : "memory");
   if (threadIdx.x == 0) {
     sm100::bar_init(qfull, 1), sm100::bar_init(qempty, 1);
     for (int i = 0; i < SLOTS; i++) sm100::bar_init(full + 8 * i, 1), sm100::bar_init(empty + 8 * i, 1);

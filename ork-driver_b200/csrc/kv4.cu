@@ -226,16 +226,16 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(Rows r, E *k, E *
 // the instructions (16 tokens of k, then 16 dims of v) and the query rows the 8 columns: a decode step has no more
 // rows than that per kv head, and the other way round half of each product would be padding.
 // First product, mma.m16n8k32 of 8-bit integers: an AND takes four codes out of a word. q is scaled per row to
-// integers below 2^20 and split into three signed bytes; the three products run one after another, the sums shifted
-// left by eight between them, and stay below 2^30: the logits carry q's 20 bits and no other error. (A code in the
+// integers below 2^21 and split into three signed bytes; the three products run one after another, the sums shifted
+// left by eight between them, and stay below 2^31: the logits carry q's 21 bits and no other error. (A code in the
 // low bits of an fp16 is an exact subnormal too, and one instruction fewer; but the tensor cores align what they add
 // by the nominal exponents, and the leading zeros cost 6 to 10 of their 24 bits: logits were off by 2^-15.)
-// Second product, mma.m16n8k16 of fp16: there those bits are to spare. A nibble in the low byte of a 16-bit half is
-// the subnormal code * 2^-24 (its low nibble) or code * 2^-20 (its high one); one AND yields two operands, and the
-// scales are taken out of the sums at the end. p * step, rounded to fp16 (11 bits; the output has no more), is
-// transposed between the products with movmatrix; a power of two per warp keeps it in range. For fp32 queries
-// (SPLIT) it is split into an fp16 and the fp16 of what that leaves, 22 bits together, the product runs twice, and
-// all codes are shifted to the top of the mantissa, code * 2^-18.
+// Second product, mma.m16n8k16 of fp16: the output has no more than 11 bits either. A shift and two ANDs put two nibbles
+// of each 16-bit half into the mantissa, as the subnormals code * 2^-22 and code * 2^-18, and the scales are taken out of
+// the sums at the end. (Left where the byte has them, a shift less, 131071 tokens came out off by 6e-4 instead of
+// 2.7e-4.) p * step, rounded to fp16, is transposed between the products with movmatrix; a power of two per warp keeps
+// it in range. For fp32 queries (SPLIT) it is split into an fp16 and the fp16 of what that leaves, 22 bits together, the
+// product runs twice, and every code is shifted to the top of the mantissa, code * 2^-18.
 // The codes of v are not negative although v has no sign: their sum would grow far above the output that it is to
 // leave after the lowest values' share is added, and the tensor cores truncate what they add. So each stage ends
 // with 8 * sum(p * step) taken out again (the sum by a product with ones, so that it holds the rounded p * step), and
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
     mx = quad_max(mx);
     const unsigned quad = 15u << (lane & 28);
     fin = (__ballot_sync(0xffffffffu, fin) & quad) == quad;
-    const int e = fin ? max(-100, min(100, 146 - (int)(__float_as_uint(mx) >> 23))) : 0;
+    const int e = fin ? max(-100, min(100, 147 - (int)(__float_as_uint(mx) >> 23))) : 0;
     const float up = pow2(e), f = fin ? a.scale * 1.4426950408889634f * pow2(-e) : __int_as_float(0x7fc00000);
     if (c == 0) qm->f[y * kRows + r] = f;
 #pragma unroll
@@ -771,8 +771,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
             af[0] = (j & 1 ? b0 >> 2 : b0 << 6) & 0x03c003c0u, af[1] = (j & 1 ? b0 >> 6 : b0 << 2) & 0x03c003c0u;
             af[2] = (j & 1 ? b1 >> 2 : b1 << 6) & 0x03c003c0u, af[3] = (j & 1 ? b1 >> 6 : b1 << 2) & 0x03c003c0u;
           } else {
-            const uint32_t s0 = j & 1 ? b0 >> 8 : b0, s1 = j & 1 ? b1 >> 8 : b1;
-            af[0] = s0 & 0x000f000fu, af[1] = s0 & 0x00f000f0u, af[2] = s1 & 0x000f000fu, af[3] = s1 & 0x00f000f0u;
+            const uint32_t s0 = j & 1 ? b0 >> 6 : b0 << 2, s1 = j & 1 ? b1 >> 6 : b1 << 2;
+            af[0] = s0 & 0x003c003cu, af[1] = s0 & 0x03c003c0u, af[2] = s1 & 0x003c003cu, af[3] = s1 & 0x03c003c0u;
           }
 #pragma unroll
           for (int y = 0; y < NT; y++) {
@@ -790,7 +790,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) o[y][g][j][i] = fmaf(sum[y][g][i & 1], SPLIT ? -0x1p-15f : i & 2 ? -0x1p-17f : -0x1p-21f, o[y][g][j][i]);
+          for (int i = 0; i < 4; i++) o[y][g][j][i] = fmaf(sum[y][g][i & 1], SPLIT || i & 2 ? -0x1p-15f : -0x1p-19f, o[y][g][j][i]);
     unit += cnt;
     __syncwarp();  // every lane has read the slot
     if (next < u1) {
@@ -809,7 +809,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   float2 *sml = reinterpret_cast<float2 *>(so + kWarps * TR * LDO);   // [kWarps][TR]
   static_assert(kWarps * TR * (LDO * 4 + 8) + 4 <= kWarps * NST * (int)sizeof(Stage<DK>), "the rings hold it");
   __syncthreads();  // the rings are idle (a warp whose wait gave up has reported it)
-  const float back = (SPLIT ? 0x1p18f : 0x1p24f) / vs, back1 = SPLIT ? back : back * 0.0625f;
+  const float back = (SPLIT ? 0x1p18f : 0x1p22f) / vs, back1 = SPLIT ? back : back * 0.0625f;
 #pragma unroll
   for (int y = 0; y < NT; y++)
 #pragma unroll

@@ -751,3 +751,18 @@ def test_prompt_store_decode_evict_decode(on):
         assert torch.equal(gk[:, h], kk[at, h]) and torch.equal(gv[:, h], vv[at, h])
     for i in range(5):
         step(d, keep + i, 300 + 3 * i, so)
+
+
+def test_the_example_runs_within_its_budget():
+    import os
+    import re
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, os.path.join(root, "examples", "long_context.py"), "--prompt", "700", "--tokens", "700",
+                        "--budget", "512", "--sequences", "3"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    held = [int(x) for x in re.search(r"tokens held \[(.*?)\]", r.stdout).group(1).split(",")]
+    # caches of 512 + 444 rounded up to 960 tokens: full after 260 of the 700 steps, down to 512, 440 more
+    assert "1 evictions" in r.stdout and held == [952] * 3 and "4.50 bits" in r.stdout
