@@ -150,7 +150,8 @@ int ork_b200_argmax_scaled_async(ork_npu *ctx, const int32_t *C, const float *bs
  * head h lies at q + r * q_ts + h * q_hs, its dk values contiguous, likewise k, v and out.
  * type ORK_B200_F16 or ORK_B200_BF16 (inputs and output); scale is positive; the scores and the output are summed in fp32 and the
  * softmax weights enter the second product rounded to `type`. Bases are 16-byte aligned, strides multiples of 8.
- * out overlaps no input. q_start, k_start: device int [nseq + 1]; q_rows / k_rows: rows that q and out / k and v
+ * out overlaps no input. The first call on a context allocates its counters (make one before capturing a CUDA graph);
+ * calls on one context run one after another. q_start, k_start: device int [nseq + 1]; q_rows / k_rows: rows that q and out / k and v
  * hold; max_q / max_k: the most rows of any one sequence (they size the launch). */
 typedef struct ork_b200_attn {
   const void *q, *k, *v;
@@ -216,7 +217,7 @@ int ork_b200_kv4_attn_async(ork_npu *ctx, const ork_b200_kv4 *c, const ork_b200_
  * slots 0.. of dst[i] [nseq][Hkv][dcap], dcap >= keep: the planes of a 4-bit cache, or of an fp32 one. No source
  * overlaps a destination. kept [nseq][Hkv][keep]: the source slots (-1 past the kept ones); score_out
  * [nseq][Hkv][dcap]: their scores (0 up to `keep`), ready to accumulate on; len_out [nseq]: min(n, keep).
- * kept, score_out and len_out may be NULL. max_len: the largest n. */
+ * kept, score_out and len_out may be NULL. max_len: the largest n. The workspace as in ork_b200_kv4_attn_async. */
 #define ORK_B200_EVICT_PLANES 8
 typedef struct ork_b200_evict {
   const float *score;
