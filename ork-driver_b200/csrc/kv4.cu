@@ -448,6 +448,26 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   Wide<DK> *wide = reinterpret_cast<Wide<DK> *>(smem + kWarps * NST * sizeof(Stage<DK>)) + warp;
   Query<DK, NT> *qm = reinterpret_cast<Query<DK, NT> *>(smem + kWarps * (NST * sizeof(Stage<DK>) + sizeof(Wide<DK>)));
   const uint32_t bars = sm100::smem_addr(qm + 1) + warp * NST * 8;
+  // q of row r of tile y, by warp y: on its way while the sequence's length is read
+  float qx[NG][16];
+  if (warp < NT) {
+    const int row = tile * TR + warp * kRows + r;
+    const E *qr = q + ((long long)s * a.T + row / G) * a.q_ts + (long long)(kvh * G + row % G) * a.q_hs + 16 * c;
+#pragma unroll
+    for (int g = 0; g < NG; g++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) qx[g][i] = 0.0f;
+    if (row < rows) {
+      auto load = [&](auto vec) {
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+          for (int i = 0; i < 16; i += 8) load8<E>(qr + 64 * g + i, decltype(vec)::value, *reinterpret_cast<float(*)[8]>(&qx[g][i]));
+      };
+      if (a.qvec) load(std::true_type());
+      else load(std::false_type());
+    }
+  }
   if (lane < NST) sm100::bar_init(bars + 8 * lane, 1);
   sm100::bar_init_fence();
   __syncwarp();
@@ -468,25 +488,17 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
       next += cnt;
     }
 
-  // q of row r of tile y, by warp y: byte 2 - d of the integers of the lane's words, even dims then odd ones
+  // as integers: byte 2 - d of those of the lane's words, even dims then odd ones
   if (warp < NT) {
-    const int y = warp, row = tile * TR + y * kRows + r;
-    const bool live = row < rows;
-    const E *qr = q + ((long long)s * a.T + row / G) * a.q_ts + (long long)(kvh * G + row % G) * a.q_hs;
-    float x[NG][16], mx = 0.0f;
+    const int y = warp;
+    float mx = 0.0f;
     bool fin = true;
 #pragma unroll
     for (int g = 0; g < NG; g++)
 #pragma unroll
-      for (int i = 0; i < 16; i += 8) {
-        float w[8] = {};
-        if (live) load8<E>(qr + 64 * g + 16 * c + i, a.qvec, w);
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          x[g][i + j] = w[j];
-          mx = fmaxf(mx, fabsf(w[j]));
-          fin = fin && fabsf(w[j]) <= 3.402823466e38f;
-        }
+      for (int i = 0; i < 16; i++) {
+        mx = fmaxf(mx, fabsf(qx[g][i]));
+        fin = fin && fabsf(qx[g][i]) <= 3.402823466e38f;
       }
     mx = quad_max(mx);
     const unsigned quad = 15u << (lane & 28);
@@ -499,7 +511,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
       int w[16], sum = 0;
 #pragma unroll
       for (int i = 0; i < 16; i++) {
-        w[i] = fin ? __float2int_rn(x[g][i] * up) : 0;
+        w[i] = fin ? __float2int_rn(qx[g][i] * up) : 0;
         sum += w[i];
         w[i] += 0x808080;  // bytes of 128 + digit
       }
@@ -862,8 +874,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
       write_row(row, d0, m, sum, v);
     }
   }
-  if (!a.join) return;
-  // few splits: the last CTA to finish joins them, in their order (more go to kv4_join_kernel, a CTA per row)
+  if (!a.join && !(WS && a.splits > 1)) return;
+  // few splits: the last CTA to finish joins them, in their order (more go to kv4_after_kernel, a CTA per row)
   unsigned int *flag = reinterpret_cast<unsigned int *>(sml + kWarps * TR);
   __threadfence();
   __syncthreads();
@@ -871,6 +883,21 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   __syncthreads();
   if (*flag != (unsigned int)a.splits - 1) return;
   __threadfence();
+  if (!a.join) {  // the rows' statistics, so that the weights need not wait for the join
+    for (int row = tile * TR + warp; row < min(rows, (tile + 1) * TR); row += kWarps) {
+      const size_t at = ((size_t)s * a.Hkv + kvh) * a.prow + row;
+      float m = -INFINITY, sum = 0.0f;
+      for (int i = lane; i < a.splits; i += 32) m = fmaxf(m, __ldcg(&a.pml[at * a.splits + i].x));
+      for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+      for (int i = lane; i < a.splits; i += 32) {
+        const float2 ml = __ldcg(a.pml + at * a.splits + i);
+        sum += ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : sm100::ex2(ml.x - m) * ml.y;
+      }
+      for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if (lane == 0) a.stat[at] = m == -INFINITY ? sum : m + log2f(sum);
+    }
+    return;
+  }
   for (int at = threadIdx.x; at < TR * DK / PER; at += 32 * kWarps) {
     const int rr = at * PER / DK, d0 = at * PER % DK, row = tile * TR + rr;
     if (row >= rows) break;
@@ -893,14 +920,15 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   }
 }
 
-// Joins the splits of one row, a CTA each.
-constexpr int kJoinThreads = 128;
+// After the attention: the first `joins` CTAs of a sequence join the splits of a row each, the others add to wsum,
+// kSumTok tokens of a kv head each: wsum[j] += sum over the rows of 2^(x_j - stat), four tokens a thread.
+constexpr int kAfter = 128, kSumTok = 4 * kAfter;
+
 template <class E, int DK>
-__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Attn4 a, E *__restrict__ out) {
-  constexpr int NW = kJoinThreads / 32, PER = DK / 32;
+__device__ __forceinline__ void join_row(const Attn4 &a, E *__restrict__ out) {
+  constexpr int NW = kAfter / 32, PER = DK / 32;
   __shared__ float2 sml[NW];
   __shared__ float so[NW][DK];
-  sm100::dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.H / a.Hkv, rows = a.T * G, s = blockIdx.y;
   const int kvh = blockIdx.x / rows, row = blockIdx.x % rows;
   const size_t pr = (((size_t)s * a.Hkv + kvh) * a.prow + row) * a.splits;
@@ -934,7 +962,6 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Attn4 a, E
 #pragma unroll
   for (int d = 0; d < PER; d++) so[warp][PER * lane + d] = v[d];
   __syncthreads();
-  sm100::dependents_launch();
   if ((int)threadIdx.x >= DK) return;
   float mm = -INFINITY, sum = 0.0f, x = 0.0f;
 #pragma unroll
@@ -946,25 +973,21 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Attn4 a, E
     if (k != 0.0f) x = fmaf(k, so[w][threadIdx.x], x);
   }
   out[(((long long)s * a.T + row / G) * a.H + kvh * G + row % G) * DK + threadIdx.x] = from_f32<E>(sum == 0.0f ? 0.0f : x / sum);
-  if (a.wsum && threadIdx.x == 0) a.stat[((size_t)s * a.Hkv + kvh) * a.prow + row] = mm == -INFINITY ? sum : mm + log2f(sum);
 }
 
-// wsum[j] += sum over the rows of 2^(x_j - stat), four tokens a thread.
-constexpr int kSumThreads = 128, kSumTok = 4 * kSumThreads;
-__global__ void __launch_bounds__(kSumThreads) kv4_wsum_kernel(const Attn4 a) {
+__device__ __forceinline__ void sum_weights(const Attn4 &a, int block) {
   constexpr int CH = 256;  // rows at a time
   __shared__ float stat[CH];
-  sm100::dependency_wait();
-  const int kvh = blockIdx.x % a.Hkv, s = blockIdx.y, rows = a.T * (a.H / a.Hkv);
+  const int kvh = block % a.Hkv, s = blockIdx.y, rows = a.T * (a.H / a.Hkv);
   const Units u = units_of(a, seq_len(a, s));
-  const int i0 = blockIdx.x / a.Hkv * kSumTok, live = u.all * kUnit, i = i0 + 4 * threadIdx.x;
+  const int i0 = block / a.Hkv * kSumTok, live = u.all * kUnit, i = i0 + 4 * threadIdx.x;
   if (i0 >= live) return;
   const size_t pr = ((size_t)s * a.Hkv + kvh) * a.prow;
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int r0 = 0; r0 < rows; r0 += CH) {
     const int r1 = min(rows, r0 + CH);
     if (r0) __syncthreads();
-    for (int row = r0 + threadIdx.x; row < r1; row += kSumThreads) stat[row - r0] = a.stat[pr + row];
+    for (int row = r0 + threadIdx.x; row < r1; row += kAfter) stat[row - r0] = a.stat[pr + row];
     __syncthreads();
     if (i < live) {
       const float *x = a.x + (pr + r0) * a.vis + i;
@@ -989,6 +1012,13 @@ __global__ void __launch_bounds__(kSumThreads) kv4_wsum_kernel(const Attn4 a) {
   if (j + 1 < u.n) w[1] += sum.y;
   if (j + 2 < u.n) w[2] += sum.z;
   if (j + 3 < u.n) w[3] += sum.w;
+}
+
+template <class E, int DK>
+__global__ void __launch_bounds__(kAfter) kv4_after_kernel(const Attn4 a, E *__restrict__ out, int joins) {
+  sm100::dependency_wait();
+  if ((int)blockIdx.x < joins) join_row<E, DK>(a, out);
+  else sum_weights(a, blockIdx.x - joins);
 }
 
 // Up to this many splits are joined by the last CTA of an item, in the launch itself; more by a CTA a row.
@@ -1024,17 +1054,12 @@ cudaError_t launch_attn_ws(const Attn4 &a, const E *q, E *out, cudaStream_t st, 
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  if (e == cudaSuccess && a.splits > 1 && !a.join) {
-    cfg.gridDim = dim3(a.Hkv * a.T * (a.H / a.Hkv), a.nseq);
-    cfg.blockDim = dim3(kJoinThreads);
+  const int joins = a.splits > 1 && !a.join ? a.Hkv * a.T * (a.H / a.Hkv) : 0;
+  if (e == cudaSuccess && (WS || joins)) {
+    cfg.gridDim = dim3(joins + (WS ? (a.vis + kSumTok - 1) / kSumTok * a.Hkv : 0), a.nseq);
+    cfg.blockDim = dim3(kAfter);
     *launches += 1;
-    e = cudaLaunchKernelEx(&cfg, kv4_join_kernel<E, DK>, a, out);
-  }
-  if (e == cudaSuccess && WS) {
-    cfg.gridDim = dim3((a.vis + kSumTok - 1) / kSumTok * a.Hkv, a.nseq);
-    cfg.blockDim = dim3(kSumThreads);
-    *launches += 1;
-    e = cudaLaunchKernelEx(&cfg, kv4_wsum_kernel, a);
+    e = cudaLaunchKernelEx(&cfg, kv4_after_kernel<E, DK>, a, out, joins);
   }
   return e;
 }
@@ -1166,7 +1191,7 @@ int ork_b200_kv4_attn_async(ork_npu *c, const ork_b200_kv4 *kv, const ork_b200_k
   const size_t mlb = whole(parts * sizeof(float2)), pob = whole(parts * kv->dk * 4), stb = a->wsum ? whole(prows * 4) : 0;
   const size_t need = mlb + pob + stb + (a->wsum ? prows * k.vis * 4 : 0);
   if (need && !grow(&c->dW, &c->capW, need)) return refuse(name, "out of device memory");
-  if (k.join) {
+  if (k.join || (a->wsum && k.splits > 1)) {
     unsigned int *z = zeroed_counts(c, (size_t)k.nseq * k.Hkv * k.tiles);
     if (!z) return refuse(name, "out of device memory");
     k.done = z + kAttnCounts;
