@@ -422,16 +422,18 @@ __device__ __forceinline__ void token_pars(const __half2 *p, float2 (&x)[NG]) {
 
 template <int DK>
 __device__ __forceinline__ void load_stage(const Attn4 &a, size_t base, const Units &u, int unit, int cnt, Stage<DK> *st,
-                                           uint32_t bar, int lane) {
+                                           uint32_t bar) {
   constexpr int NG = DK / kGroup;
   const size_t tok = base + (size_t)token_of(u, unit);
   const uint32_t cb = (uint32_t)cnt * kUnit * (DK / 2), pb = (uint32_t)cnt * kUnit * NG * 4;
-  if (lane == 0) sm100::bar_expect(bar, 2 * cb + 2 * pb);
+  if (sm100::elect_one()) {
+    sm100::bar_expect(bar, 2 * cb + 2 * pb);
+    sm100::bulk_load(sm100::smem_addr(st->k), a.kc + tok * (DK / 2), cb, bar);
+    sm100::bulk_load(sm100::smem_addr(st->kp), a.kp + tok * NG * 2, pb, bar);
+    sm100::bulk_load(sm100::smem_addr(st->v), a.vc + tok * (DK / 2), cb, bar);
+    sm100::bulk_load(sm100::smem_addr(st->vp), a.vp + tok * NG * 2, pb, bar);
+  }
   __syncwarp();
-  if (lane == 0) sm100::bulk_load(sm100::smem_addr(st->k), a.kc + tok * (DK / 2), cb, bar);
-  else if (lane == 1) sm100::bulk_load(sm100::smem_addr(st->kp), a.kp + tok * NG * 2, pb, bar);
-  else if (lane == 2) sm100::bulk_load(sm100::smem_addr(st->v), a.vc + tok * (DK / 2), cb, bar);
-  else if (lane == 3) sm100::bulk_load(sm100::smem_addr(st->vp), a.vp + tok * NG * 2, pb, bar);
 }
 
 // NT column tiles of kRows query rows share every operand made from the codes.
@@ -472,7 +474,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   sm100::bar_init_fence();
   __syncwarp();
 
-  const int n = seq_len(a, s);
+  const int n = sm100::uniform(seq_len(a, s));
   const Units u = units_of(a, n);
   const int cu0 = (int)((long long)u.all * split / a.splits), cu1 = (int)((long long)u.all * (split + 1) / a.splits);
   const int u0 = cu0 + (cu1 - cu0) * warp / kWarps, u1 = cu0 + (cu1 - cu0) * (warp + 1) / kWarps;
@@ -484,7 +486,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   for (int i = 0; i < NST; i++)
     if (next < u1) {
       const int cnt = count(next);
-      load_stage<DK>(a, base, u, next, cnt, ring + i, bars + 8 * i, lane);
+      load_stage<DK>(a, base, u, next, cnt, ring + i, bars + 8 * i);
       next += cnt;
     }
 
@@ -807,7 +809,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
     __syncwarp();  // every lane has read the slot
     if (next < u1) {
       const int more = count(next);
-      load_stage<DK>(a, base, u, next, more, ring + slot, bars + 8 * slot, lane);
+      load_stage<DK>(a, base, u, next, more, ring + slot, bars + 8 * slot);
       next += more;
     }
     if (++slot == NST) slot = 0, parity ^= 1;
