@@ -33,14 +33,17 @@ __device__ __forceinline__ void kv4_error() {
 }
 
 // ---- rows into the cache and back ------------------------------------------------------------------------------
-// A thread handles 8 consecutive dims of k or of v of one row and head, one 32-bit word of codes: a group's 8 threads
-// find its lowest and largest value with three shuffles, and dk / 4 threads read and write a token's k and v of a head
-// whole. A warp keeps its heads and steps through the rows of its sequence (blockIdx.y).
+// A storing thread handles 16 consecutive dims of k or of v of one row and head, two 32-bit words of codes: a group's 4
+// threads find its lowest and largest value with two shuffles, and dk / 8 threads read and write a token's k and v of a
+// head whole; its next row is on the way as it lies in memory. A reading-back thread handles one word, four rows at a
+// time. A warp keeps its heads and steps through the rows of its sequence (blockIdx.y).
 // The division by the step, which has to be the IEEE one for the codes to be the definition's, is a product with the
 // step's reciprocal wherever that is sure to round to the same code, and is done again where it is not (a quotient within
 // 1e-5 of the middle between two codes; the product is off by 6e-6 at most).
-// Bound by memory: the store of 49145 rows of 8 heads of 128 bf16 dims reads 201 MB and writes 57 MB (100 us, the load back 50 us; issue slots 65 % used).
+// 49145 rows of 8 heads of 128 bf16 dims: the store reads 201 MB and writes 57 MB in 70 us, 3.7 TB/s, bound by its
+// instructions (75 % of the issue slots: lowest, largest, quotients); the load back 46 us, 5.5 TB/s, bound by memory.
 constexpr int kRowThreads = 256;
+constexpr int kStoreWords = 2;  // words of codes that a storing thread makes; one: 84 us instead of 70
 
 struct Rows {
   int nseq, Hkv, cap, rows;
@@ -64,26 +67,43 @@ __device__ __forceinline__ uint32_t narrow2(float x, float y, const __nv_bfloat1
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 template <class E>
-__device__ __forceinline__ void load8(const E *p, bool vec, float (&x)[8]) {
+struct Raw8 {  // eight values as they lie in memory
+  uint32_t w[2 * sizeof(E)];
+};
+template <class E>
+__device__ __forceinline__ void load8(const E *p, bool vec, Raw8<E> &x) {
   if (vec) {
-    const uint4 a = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-    if constexpr (sizeof(E) == 4) {
-      const float4 c = *reinterpret_cast<const float4 *>(p + 4);
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[i] = __uint_as_float(w[i]);
-      x[4] = c.x, x[5] = c.y, x[6] = c.z, x[7] = c.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float2 f = widen2(w[i], p);
-        x[2 * i] = f.x, x[2 * i + 1] = f.y;
-      }
+    for (int i = 0; i < (int)sizeof(E) / 2; i++) {
+      const uint4 a = reinterpret_cast<const uint4 *>(p)[i];
+      x.w[4 * i] = a.x, x.w[4 * i + 1] = a.y, x.w[4 * i + 2] = a.z, x.w[4 * i + 3] = a.w;
     }
-  } else {
+  } else if constexpr (sizeof(E) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = to_f32(p[i]);
+    for (int i = 0; i < 8; i++) x.w[i] = __float_as_uint(p[i]);
+  } else {
+    const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; i++) x.w[i] = h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
   }
+}
+template <class E>
+__device__ __forceinline__ void widen8(const Raw8<E> &r, float *x) {
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(E) * 2; i++) {
+    if constexpr (sizeof(E) == 4) {
+      x[i] = __uint_as_float(r.w[i]);
+    } else {
+      const float2 f = widen2(r.w[i], (const E *)nullptr);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  }
+}
+template <class E>
+__device__ __forceinline__ void load8(const E *p, bool vec, float (&x)[8]) {
+  Raw8<E> r;
+  load8(p, vec, r);
+  widen8(r, x);
 }
 template <class E>
 __device__ __forceinline__ void store8(E *p, bool vec, const float (&x)[8]) {
@@ -113,9 +133,10 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
 }
 
 template <class E, int DK, bool STORE, bool VEC>
-__global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(Rows r, E *k, E *v, uint32_t *kc, uint32_t *vc,
+__global__ void __launch_bounds__(kRowThreads, STORE ? 4 : 1) kv4_rows_kernel(Rows r, E *k, E *v, uint32_t *kc, uint32_t *vc,
                                                                __half2 *kp, __half2 *vp) {
-  constexpr int WORDS = DK / 8, LANES = 2 * WORDS;  // words of a row; threads of a (row, head): k's, then v's
+  constexpr int WORDS = DK / 8, NW = STORE ? kStoreWords : 1;  // words of a row, of a thread
+  constexpr int LANES = 2 * WORDS / NW;                             // threads of a (row, head): k's, then v's
   const int s = blockIdx.y, lane = threadIdx.x & 31;
   const int row0 = r.start ? r.start[s] : s * r.rows;
   const int n = r.start ? r.start[s + 1] - row0 : r.rows;
@@ -123,8 +144,8 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(Rows r, E *k, E *
   // teams of LANES threads: team i takes head i % Hkv and every `step`-th row from i / Hkv on
   const int teams = gridDim.x * (kRowThreads / LANES), step = teams / r.Hkv;
   const int team = (blockIdx.x * kRowThreads + threadIdx.x) / LANES, h = team % r.Hkv, t0 = team / r.Hkv;
-  const int at = threadIdx.x % LANES, w = at % WORDS;
-  const bool is_v = at >= WORDS;
+  const int at = threadIdx.x % LANES, w = at * NW % WORDS;
+  const bool is_v = at * NW >= WORDS;
   if (t0 >= step) return;  // whole teams; a group's threads stay together
   // the rows whose slots the cache has
   const long long first = slot0 < 0 ? -(long long)slot0 : 0, end = (long long)r.cap - slot0;
@@ -137,8 +158,9 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(Rows r, E *k, E *
   const size_t tok = ((size_t)s * r.Hkv + h) * r.cap + (size_t)((long long)slot0 + t);
   uint32_t *code = (is_v ? vc : kc) + tok * WORDS + w;
   __half2 *par = (is_v ? vp : kp) + tok * (DK / kGroup) + w / 8;
-  const unsigned mask = 0xffu << (lane & 24);
-  float next[8];
+  constexpr int GROUP = 8 / NW;  // threads of a group of 64 dims
+  const unsigned mask = ((1u << GROUP) - 1) << (lane & ~(GROUP - 1));
+  Raw8<E> next[NW];
   if constexpr (!STORE) {  // four rows at a time on their way: a row is little to ask for
     for (; t < last; t += 4 * step, row += 4 * hop, code += 4 * step * WORDS, par += 4 * step * (DK / kGroup)) {
       uint32_t c[4];
@@ -159,17 +181,23 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(Rows r, E *k, E *
     }
     return;
   }
-  if (STORE && t < last) load8<E>(row, VEC, next);
+  if (STORE && t < last)
+#pragma unroll
+    for (int u = 0; u < NW; u++) load8<E>(row + 8 * u, VEC, next[u]);
   for (; t < last; t += step, row += hop, code += step * WORDS, par += step * (DK / kGroup)) {
-    float x[8];
+    float x[NW][8];
     if constexpr (STORE) {
+      widen8(next[0], x[0]);
+      float lo = x[0][0], hi = lo;
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = next[i];
-      if (t + step < last) load8<E>(row + hop, VEC, next);
-      float lo = min_nan(min_nan(x[0], x[1], x[2]), min_nan(x[3], x[4], x[5]), min_nan(x[6], x[7], x[7]));
-      float hi = max_nan(max_nan(x[0], x[1], x[2]), max_nan(x[3], x[4], x[5]), max_nan(x[6], x[7], x[7]));
+      for (int u = 0; u < NW; u++) {
+        if (u) widen8(next[u], x[u]);
+        if (t + step < last) load8<E>(row + hop + 8 * u, VEC, next[u]);
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) {
+        for (int i = 0; i < 8; i += 2) lo = min_nan(lo, x[u][i], x[u][i + 1]), hi = max_nan(hi, x[u][i], x[u][i + 1]);
+      }
+#pragma unroll
+      for (int o = 1; o < GROUP; o <<= 1) {
         const float l2 = __shfl_xor_sync(mask, lo, o), h2 = __shfl_xor_sync(mask, hi, o);
         lo = min_nan(lo, l2, l2);
         hi = max_nan(hi, h2, h2);
@@ -179,41 +207,43 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(Rows r, E *k, E *
       __half low = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
       if (!(fabsf(lo) <= 3.402823466e38f && fabsf(hi) <= 3.402823466e38f)) step2 = low = __ushort_as_half((unsigned short)0x7fff);
       const float sf = __half2float(step2), lf = __half2float(low);
-      uint32_t c;
-      {
+      float inv = 0.0f;  // no step, no codes
+      if (sf > 0.0f) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf * 15.0f));
+      uint32_t c[NW];
+#pragma unroll
+      for (int u = 0; u < NW; u++) {
         using namespace sm100;
-        float inv = 0.0f;  // no step, no codes
-        if (sf > 0.0f) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf * 15.0f));
         const float2 two23 = both(8388608.0f);
         float off = 0.0f, r4[8];
         float2 m[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           // the quotient over 15 clamped to [0, 1]; m: the code plus 2^23, rounded to an integer by that addition
-          const float2 d = add2(make_float2(x[2 * i], x[2 * i + 1]), both(-lf));
+          const float2 d = add2(make_float2(x[u][2 * i], x[u][2 * i + 1]), both(-lf));
           const float2 q = make_float2(__saturatef(d.x * inv), __saturatef(d.y * inv));
           m[i] = fma2(q, both(15.0f), two23);
           const float2 z = add2(m[i], both(-8388608.0f));
-          const float2 e = fma2(q, both(15.0f), mul2(z, both(-1.0f)));
+          const float2 e = fma2(q, both(-15.0f), z);
           off = fmaxf(off, fmaxf(fabsf(e.x), fabsf(e.y)));
           r4[2 * i] = z.x, r4[2 * i + 1] = z.y;
         }
         // four codes side by side in the low bits of 2^23 + c0 + 16 c1 + 256 c2 + 4096 c3
         const float a = fmaf(r4[3], 4096.0f, fmaf(r4[2], 256.0f, fmaf(r4[1], 16.0f, m[0].x)));
         const float b = fmaf(r4[7], 4096.0f, fmaf(r4[6], 256.0f, fmaf(r4[5], 16.0f, m[2].x)));
-        c = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x5410);
+        c[u] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x5410);
         if (off > 0.49999f) {
-          c = 0;
+          c[u] = 0;
 #pragma unroll 1
           for (int i = 0; i < 8; i++) {
-            float y = x[0];
+            float y = x[u][0];
 #pragma unroll
-            for (int j = 1; j < 8; j++) y = i == j ? x[j] : y;
-            c |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(y, lf), sf)), 0.0f), 15.0f) << (4 * i);
+            for (int j = 1; j < 8; j++) y = i == j ? x[u][j] : y;
+            c[u] |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(y, lf), sf)), 0.0f), 15.0f) << (4 * i);
           }
         }
       }
-      *code = c;
+      if constexpr (NW == 2) *reinterpret_cast<uint2 *>(code) = make_uint2(c[0], c[1]);
+      else *code = c[0];
       if ((w & 7) == 0) *par = __halves2half2(step2, low);
     }
   }
@@ -1117,9 +1147,12 @@ static int kv4_rows(ork_npu *c, const ork_b200_kv4 *kv, const void *k, const voi
   if (rows == 0) return 0;
   const bool vec = ((uintptr_t)k | (uintptr_t)v | (size_t)ts * es | (size_t)hs * es) % 16 == 0;
   const Rows r = {kv->nseq, kv->Hkv, kv->cap, rows, ts, hs, start, pos};
-  // teams of a (row, head): a multiple of Hkv, so that every thread has a head; about 8 blocks an SM
-  const long long per = kRowThreads / (kv->dk / 4), want = ((long long)rows * kv->Hkv + per - 1) / per;
-  const long long most = std::max<long long>(148LL * 8 / kv->nseq, (kv->Hkv + per - 1) / per);
+  // Teams of a (row, head): a multiple of Hkv, so that every thread has a head; as many rows for each as it has on their
+  // way at once, and 12 blocks an SM at most (three waves of a store: 8 are 1 to 4 % slower, one row for each 15 to 30 %
+  // on 4000 rows of 64 dims).
+  const long long per = kRowThreads / (kv->dk / 4 / (store ? kStoreWords : 1)), each = store ? 2 : 4;
+  const long long want = ((rows + each - 1) / each * kv->Hkv + per - 1) / per;
+  const long long most = std::max<long long>(148LL * 12 / kv->nseq, (kv->Hkv + per - 1) / per);
   const dim3 grid((unsigned)std::min(want, most), kv->nseq);
   const cudaError_t e = with_elem(type, [&](auto *t) {
     using E = std::remove_pointer_t<decltype(t)>;
