@@ -3,7 +3,7 @@
 // A token's key orders it: the first `sinks` and last `recent` tokens have the largest key, others their score's
 // bits mapped to an unsigned word of the same order (a NaN's: minus infinity's). The kept ones are those above a threshold
 // key, and of those equal to it the lowest slots. Two launches:
-//   evict_pick  a cluster of CTAs per (sequence, kv head) finds the threshold eight bits at a time: each pass counts the
+//   evict_pick  a cluster of CTAs per (sequence, kv head) finds the threshold in three digits of 11, 11 and 10 bits: each pass counts the
 //               keys that share the bits found so far, every CTA of its part of the tokens, and adds the counts up through
 //               distributed shared memory. Keys stay in shared memory between the passes when they fit. It ends with the
 //               number of kept tokens, and of kept ones equal to the threshold, before each chunk of kChunk tokens.
@@ -29,8 +29,13 @@ namespace {
 
 constexpr int kThreads = 1024;  // of evict_pick
 constexpr int kChunk = 512;     // tokens of a CTA of evict_move, one a thread
+// Words that a thread of evict_move has on their way: two, and four CTAs an SM, whose 32 registers a thread leave no more.
+// 16 x 8 heads of up to 32768 4-bit tokens, moved and read back: 239 us; four words and three CTAs 242, eight and two 258.
+constexpr int kMoves = 2;
 constexpr int kCluster = 8;     // CTAs that pick together, at most
 constexpr int kHeld = 24576;    // keys that a CTA of evict_pick holds
+constexpr int kDigits = 2048;   // of a pass, two a thread: 11, 11 and 10 bits
+static_assert(kDigits == 2 * kThreads);
 
 // What evict_pick leaves for evict_move, per (sequence, kv head): the threshold, how many of those equal to it are kept,
 // and per chunk the kept tokens above it and those equal to it before the chunk.
@@ -67,6 +72,13 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int2 remote_int2(const int *p, uint32_t rank) {
+  uint32_t at;
+  int2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(sm100::smem_addr(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
 }
 __device__ __forceinline__ int remote_int(const int *p, uint32_t rank) {
   uint32_t at;
@@ -105,7 +117,8 @@ __device__ __forceinline__ int block_scan(int v, int *red, int *total) {
 // blockIdx.y: (sequence, kv head); the CTAs of its cluster take runs of whole chunks of its tokens.
 __global__ void __launch_bounds__(kThreads) evict_pick(const ork_b200_evict e, Picked *picked, int2 *before, int chunks, int hold) {
   extern __shared__ uint32_t keys[];
-  __shared__ int hist[2][256], sum[256], red[32], ends[2];
+  __shared__ __align__(8) int hist[2][kDigits];
+  __shared__ int sum[128], red[32], ends[2];
   __shared__ int s_digit, s_left;
   const int sh = blockIdx.y, tid = threadIdx.x;
   const uint32_t rank = cluster_rank(), size = cluster_size();
@@ -117,10 +130,10 @@ __global__ void __launch_bounds__(kThreads) evict_pick(const ork_b200_evict e, P
   uint32_t prefix = 0;
   int left = m;  // of the keys that share the prefix, how many are kept
   if (n > m) {
-    for (int pass = 0; pass < 4; pass++) {
-      const int shift = 24 - 8 * pass;
+    for (int pass = 0; pass < 3; pass++) {
+      const int bits = pass < 2 ? 11 : 10, shift = max(0, 21 - 11 * pass);
       int *h = hist[pass & 1];  // the other one may still be read by a CTA that is behind
-      for (int i = tid; i < 256; i += kThreads) h[i] = 0;
+      reinterpret_cast<int2 *>(h)[tid] = make_int2(0, 0);
       __syncthreads();
       for (int b = j0; b < j1; b += 8 * kThreads) {
         uint32_t ks[8];
@@ -133,46 +146,28 @@ __global__ void __launch_bounds__(kThreads) evict_pick(const ork_b200_evict e, P
         for (int u = 0; u < 8; u++) {
           const int j = b + u * kThreads + tid;
           if (b + u * kThreads >= j1) break;
-          bool in = j < j1;
+          if (j >= j1) continue;
           uint32_t k = ks[u];
-          if (in) {
-            if (pass == 0 || !hold) k = key_of(__uint_as_float(k), j, n, e.sinks, e.recent);
-            if (pass == 0 && hold) keys[j - j0] = k;
-            in = pass == 0 || (k >> (shift + 8)) == (prefix >> (shift + 8));
-          }
-          // one addition for the lanes that share a digit with the first: most scores share their top bits (with
-          // match.any, an addition for every digit, 47 us instead of 40 for 128 x 32768 scores)
-          const unsigned who = __ballot_sync(0xffffffffu, in);
-          if (who) {
-            const int d = (k >> shift) & 255, lead = __shfl_sync(0xffffffffu, d, __ffs(who) - 1);
-            const unsigned same = __ballot_sync(0xffffffffu, in && d == lead);
-            if ((tid & 31) == __ffs(who) - 1) atomicAdd(&h[lead], __popc(same));
-            else if (in && d != lead) atomicAdd(&h[d], 1);
-          }
+          if (pass == 0 || !hold) k = key_of(__uint_as_float(k), j, n, e.sinks, e.recent);
+          if (pass == 0 && hold) keys[j - j0] = k;
+          // an addition each, equal digits or not: one for the lanes that share one, found by ballots, was slower even
+          // with every score the same (253 us the whole call instead of 245)
+          if (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&h[(k >> shift) & ((1 << bits) - 1)], 1);
         }
       }
       __syncthreads();
       if (size > 1) cluster_sync();
-      if (tid < 256) {
-        int v = h[tid];
-        for (uint32_t q = 1; q < size; q++) v += remote_int(&h[tid], (rank + q) % size);
-        sum[tid] = v;
+      const int d = kDigits - 2 - 2 * tid;  // this thread's digits: d + 1, then d
+      int2 v = *reinterpret_cast<const int2 *>(&h[d]);
+      for (uint32_t q = 1; q < size; q++) {
+        const int2 o = remote_int2(&h[d], (rank + q) % size);
+        v.x += o.x, v.y += o.y;
       }
-      __syncthreads();
-      if (tid < 32) {  // lane l: digits 255 - 8 l down to 248 - 8 l
-        int mine = 0;
-        for (int i = 0; i < 8; i++) mine += sum[255 - 8 * tid - i];
-        int above = mine;
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, above, o);
-          if (tid >= o) above += y;
-        }
-        above -= mine;
-        if (above < left && above + mine >= left) {
-          int d = 255 - 8 * tid;
-          for (; above + sum[d] < left; d--) above += sum[d];
-          s_digit = d, s_left = left - above;
-        }
+      int all_of;
+      const int above = block_scan(v.x + v.y, red, &all_of);
+      if (above < left && above + v.x + v.y >= left) {
+        const bool low = above + v.y < left;
+        s_digit = low ? d : d + 1, s_left = left - above - (low ? v.y : 0);
       }
       __syncthreads();
       prefix |= (uint32_t)s_digit << shift;
@@ -225,7 +220,7 @@ __global__ void __launch_bounds__(kThreads) evict_pick(const ork_b200_evict e, P
 // blockIdx.x: a chunk of the tokens of (sequence, kv head) blockIdx.y; the grid also covers the budget, whose unused
 // places are filled. gridDim.z CTAs share a chunk's copies where there are few chunks (wide rows of one chat: 8 of them
 // took a chunk's 512 rows of 512 bytes from 16 us to 12 us).
-__global__ void __launch_bounds__(kChunk) evict_move(const ork_b200_evict e, const Picked *picked, const int2 *before, int chunks) {
+__global__ void __launch_bounds__(kChunk, 4) evict_move(const ork_b200_evict e, const Picked *picked, const int2 *before, int chunks) {
   __shared__ int red[32], from[kChunk];
   sm100::dependency_wait();
   const int sh = blockIdx.y, tid = threadIdx.x, c = blockIdx.x;
@@ -265,15 +260,15 @@ __global__ void __launch_bounds__(kChunk) evict_move(const ork_b200_evict e, con
       const int words = bytes / (int)sizeof(W), items = total * words;
       const bool shifts = (words & (words - 1)) == 0;
       const int by = __ffs(words) - 1;
-      for (int i0 = i00; i0 < items; i0 += 8 * hop) {
-        W v[8];
+      for (int i0 = i00; i0 < items; i0 += kMoves * hop) {
+        W v[kMoves];
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
+        for (int u = 0; u < kMoves; u++) {
           const int i = i0 + u * hop, row = shifts ? i >> by : i / words;
           if (i < items) v[u] = reinterpret_cast<const W *>(src + (size_t)from[row] * bytes)[i - row * words];
         }
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
+        for (int u = 0; u < kMoves; u++) {
           const int i = i0 + u * hop;
           if (i < items) reinterpret_cast<W *>(dst)[i] = v[u];
         }
