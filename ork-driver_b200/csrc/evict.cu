@@ -218,8 +218,8 @@ __global__ void __launch_bounds__(kThreads) evict_pick(const ork_b200_evict e, P
 }
 
 // blockIdx.x: a chunk of the tokens of (sequence, kv head) blockIdx.y; the grid also covers the budget, whose unused
-// places are filled. gridDim.z CTAs share a chunk's copies where there are few chunks (wide rows of one chat: 8 of them
-// took a chunk's 512 rows of 512 bytes from 16 us to 12 us).
+// places are filled. gridDim.z CTAs share a chunk's copies where there are few chunks (wide rows of one chat,
+// 4001 tokens of 8 heads of 512 bytes: 16.5 us the call instead of 22.6).
 __global__ void __launch_bounds__(kChunk, 4) evict_move(const ork_b200_evict e, const Picked *picked, const int2 *before, int chunks) {
   __shared__ int red[32], from[kChunk];
   sm100::dependency_wait();

@@ -271,6 +271,11 @@ __global__ void __launch_bounds__(kRowThreads, STORE ? 4 : 1) kv4_rows_kernel(Ro
 // with 8 * sum(p * step) taken out again (the sum by a product with ones, so that it holds the rounded p * step), and
 // v is (c - 8) s + (b + 8 s).
 //
+// Bound by the instructions on the codes: 17.6 a token and kv head, issue slots 60 % and the tensor pipe 38 % used, at
+// 4.8 to 5.3 TB/s of cache (55 x 8 heads of 16384 bf16 tokens, 8 rows each: 197 us; the copies alone run at 6.4 TB/s).
+// Stages are requested by one elected lane at addresses that are the same in a warp by construction (uniform
+// registers): 13 % faster than a lane picked by its number.
+//
 // A warp owns a run of 16-token units and brings kStageUnits of them at a time into its own ring of shared memory
 // with bulk copies (codes and parameters of k and v, contiguous); no other warp waits on it. The parameters are
 // widened to fp32 once per stage (each token's are needed by four lanes). Softmax is kept online per stage. The warps
@@ -1057,8 +1062,9 @@ __global__ void __launch_bounds__(kAfter) kv4_after_kernel(const Attn4 a, E *__r
 constexpr int kJoinSplits = 16;
 
 // Token splits: the fewest waves of resident CTAs times what one takes, its units and about 45 units' worth (9 us) of
-// setting up and joining, fitted to 440 items of 1024 units in one wave (215 us) to four (242 us), 296 items (3 splits,
-// two waves, 159 us; 1 split 171 us, 6 splits 176 us) and 8 items of 8192 units (55 splits 58 us, 37 62 us, 74 69 us).
+// setting up and joining. Measured: 440 items of 1024 units 197, 203, 210, 215 us in 1 to 4 splits, 231 in 8; 296 items
+// 142, 159, 143, 149 us in 1 to 4, 160 in 6; 144 items 104, 79, 76, 95 us in 1 to 4; 8 items of 8192 units 69 us in 18
+// splits, 58 in 37 and 55, 66 in 74. It picks 1, 3, 3 and 55.
 // Two units a warp at least.
 int choose_splits(const Attn4 &a, int ctas) {
   const long long items = (long long)a.nseq * a.Hkv * a.tiles, units = a.vis / kUnit, slots = 148LL * ctas;
