@@ -1020,35 +1020,37 @@ __device__ __forceinline__ void sum_weights(const Attn4 &a, int block) {
   const int i0 = block / a.Hkv * kSumTok, live = u.all * kUnit, i = i0 + 4 * threadIdx.x;
   if (i0 >= live) return;
   const size_t pr = ((size_t)s * a.Hkv + kvh) * a.prow;
-  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const int j = i < live ? token_of(u, i / kUnit) + i % kUnit : u.n;
+  float *w = a.wsum + ((size_t)s * a.Hkv + kvh) * a.cap + j;
+  float old[4], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int e = 0; e < 4; e++) old[e] = j + e < u.n ? w[e] : 0.0f;
   for (int r0 = 0; r0 < rows; r0 += CH) {
     const int r1 = min(rows, r0 + CH);
     if (r0) __syncthreads();
     for (int row = r0 + threadIdx.x; row < r1; row += kAfter) stat[row - r0] = a.stat[pr + row];
-    __syncthreads();
-    if (i < live) {
-      const float *x = a.x + (pr + r0) * a.vis + i;
-#pragma unroll 8
-      for (int row = 0; row < r1 - r0; row++) {
-        const float4 v = __ldcs(reinterpret_cast<const float4 *>(x + (size_t)row * a.vis));
-        const float st = stat[row];  // a place that is not visible holds -inf
-        if (st != st) {              // a row that sees a NaN: so are its weights, of what it sees
-          auto add = [&](float &t, float y) { if (y != -INFINITY) t = st; };
-          add(sum.x, v.x), add(sum.y, v.y), add(sum.z, v.z), add(sum.w, v.w);
-          continue;
+    for (int b = r0; b < r1; b += 8) {  // eight rows on their way at once
+      const float *x = a.x + (pr + b) * a.vis + i;
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (b + k < r1 && i < live) v[k] = __ldcs(reinterpret_cast<const float4 *>(x + (size_t)k * a.vis));
+      if (b == r0) __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        if (b + k >= r1 || i >= live) break;
+        const float st = stat[b + k - r0], y[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {  // a place that is not visible holds -inf
+          if (st == st) sum[e] += sm100::ex2(y[e] - st);
+          else if (y[e] != -INFINITY) sum[e] = st;  // a row that sees a NaN: so are its weights, of what it sees
         }
-        sum.x += sm100::ex2(v.x - st), sum.y += sm100::ex2(v.y - st);
-        sum.z += sm100::ex2(v.z - st), sum.w += sm100::ex2(v.w - st);
       }
     }
   }
-  if (i >= live) return;
-  const int j = token_of(u, i / kUnit) + i % kUnit;
-  float *w = a.wsum + ((size_t)s * a.Hkv + kvh) * a.cap + j;
-  if (j < u.n) w[0] += sum.x;
-  if (j + 1 < u.n) w[1] += sum.y;
-  if (j + 2 < u.n) w[2] += sum.z;
-  if (j + 3 < u.n) w[3] += sum.w;
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (j + e < u.n) w[e] = old[e] + sum[e];
 }
 
 template <class E, int DK>
