@@ -958,7 +958,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
 }
 
 // After the attention: the first `joins` CTAs of a sequence join the splits of a row each, the others add to wsum,
-// kSumTok tokens of a kv head each: wsum[j] += sum over the rows of 2^(x_j - stat), four tokens a thread.
+// kSumTok tokens of a kv head each: wsum[j] += sum over the rows of 2^(x_j - stat), four tokens a thread, four rows on
+// their way at once (64 rows of 131071 logits, the whole pass: 53 us; eight rows and fewer CTAs an SM 55, one 57).
 constexpr int kAfter = 128, kSumTok = 4 * kAfter;
 
 template <class E, int DK>
@@ -1029,15 +1030,15 @@ __device__ __forceinline__ void sum_weights(const Attn4 &a, int block) {
     const int r1 = min(rows, r0 + CH);
     if (r0) __syncthreads();
     for (int row = r0 + threadIdx.x; row < r1; row += kAfter) stat[row - r0] = a.stat[pr + row];
-    for (int b = r0; b < r1; b += 8) {  // eight rows on their way at once
+    for (int b = r0; b < r1; b += 4) {  // four rows on their way at once
       const float *x = a.x + (pr + b) * a.vis + i;
-      float4 v[8];
+      float4 v[4];
 #pragma unroll
-      for (int k = 0; k < 8; k++)
+      for (int k = 0; k < 4; k++)
         if (b + k < r1 && i < live) v[k] = __ldcs(reinterpret_cast<const float4 *>(x + (size_t)k * a.vis));
       if (b == r0) __syncthreads();
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
+      for (int k = 0; k < 4; k++) {
         if (b + k >= r1 || i >= live) break;
         const float st = stat[b + k - r0], y[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
