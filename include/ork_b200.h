@@ -216,8 +216,8 @@ int ork_b200_kv4_attn_async(ork_npu *ctx, const ork_b200_kv4 *c, const ork_b200_
  * order, from each of `nplanes` source planes src[i] [nseq][Hkv][cap] rows of row_bytes[i] (a multiple of 4, at most 65536) to
  * slots 0.. of dst[i] [nseq][Hkv][dcap], dcap >= keep: the planes of a 4-bit cache, or of an fp32 one. No source
  * overlaps a destination. kept [nseq][Hkv][keep]: the source slots (-1 past the kept ones); score_out
- * [nseq][Hkv][dcap]: their scores (0 up to `keep`), ready to accumulate on; len_out [nseq]: min(n, keep).
- * kept, score_out and len_out may be NULL. max_len: the largest n. The workspace as in ork_b200_kv4_attn_async. */
+ * [nseq][Hkv][dcap]: their scores (0 up to `keep`), ready to accumulate on; len_out [nseq]: min(n, keep); it may be
+ * len itself. kept, score_out and len_out may be NULL. max_len: the largest n. The workspace as in ork_b200_kv4_attn_async. */
 #define ORK_B200_EVICT_PLANES 8
 typedef struct ork_b200_evict {
   const float *score;

@@ -210,10 +210,7 @@ __global__ void __launch_bounds__(kThreads) evict_pick(const ork_b200_evict e, P
     for (int c = c0 + tid; c < c1; c += kThreads) out[c].x += a, out[c].y += q;
     cluster_sync();  // nobody leaves while another may read its shared memory
   }
-  if (rank == 0 && tid == 0) {
-    picked[sh] = Picked{n > m ? prefix : 0u, n > m ? left : 0, n, 0};
-    if (e.len_out && sh % e.Hkv == 0) e.len_out[sh / e.Hkv] = m;
-  }
+  if (rank == 0 && tid == 0) picked[sh] = Picked{n > m ? prefix : 0u, n > m ? left : 0, n, 0};
   sm100::dependents_launch();
 }
 
@@ -229,6 +226,8 @@ __global__ void __launch_bounds__(kChunk, 4) evict_move(const ork_b200_evict e, 
   const Picked p = picked[sh];
   const int n = p.n, m = min(n, e.keep);
   const bool tell = blockIdx.z == 0;
+  // the lengths are written here, where nothing reads them any more: len_out may be len
+  if (tell && c == 0 && tid == 0 && e.len_out && sh % e.Hkv == 0) e.len_out[sh / e.Hkv] = m;
   if (tell && j < e.keep && j >= m) {
     if (e.kept) e.kept[(size_t)sh * e.keep + j] = -1;
     if (e.score_out) e.score_out[(size_t)sh * e.dcap + j] = 0.0f;
