@@ -136,7 +136,10 @@ int ork_b200_argmax_scaled_async(ork_npu *ctx, const int32_t *C, const float *bs
  * No counterpart in ork-driver, whose attention is the decode layer's over one fp32 cache. All calls take device
  * pointers, enqueue on the context's stream and return 0, or -1 with a message and nothing queued. What only the
  * device can see (a length or slot outside its cache) skips that sequence or row and is reported by the next
- * ork_b200_sync. `type` is one of the three below; strides are in elements. Head size dk is 64 or 128; query head
+ * ork_b200_sync. Calls on one context share a workspace and counters, which the first call of a larger size allocates:
+ * they run one after another, and one call of each size is made before a CUDA graph captures it (a capture that would
+ * need more is refused). What a captured call was given stays allocated until the context is freed, so that its graph
+ * can be replayed whatever is called in between. `type` is one of the three below; strides are in elements. Head size dk is 64 or 128; query head
  * h reads kv head h / (H / Hkv), so H is a multiple of Hkv. */
 #define ORK_B200_F32 0
 #define ORK_B200_F16 1
@@ -150,8 +153,7 @@ int ork_b200_argmax_scaled_async(ork_npu *ctx, const int32_t *C, const float *bs
  * head h lies at q + r * q_ts + h * q_hs, its dk values contiguous, likewise k, v and out.
  * type ORK_B200_F16 or ORK_B200_BF16 (inputs and output); scale is positive; the scores and the output are summed in fp32 and the
  * softmax weights enter the second product rounded to `type`. Bases are 16-byte aligned, strides multiples of 8.
- * out overlaps no input. The first call on a context allocates its counters (make one before capturing a CUDA graph);
- * calls on one context run one after another. q_start, k_start: device int [nseq + 1]; q_rows / k_rows: rows that q and out / k and v
+ * out overlaps no input. q_start, k_start: device int [nseq + 1]; q_rows / k_rows: rows that q and out / k and v
  * hold; max_q / max_k: the most rows of any one sequence (they size the launch). */
 typedef struct ork_b200_attn {
   const void *q, *k, *v;
@@ -195,8 +197,7 @@ int ork_b200_kv4_load_async(ork_npu *ctx, const ork_b200_kv4 *c, void *k, void *
  * three, and are aligned to it; arithmetic is fp32-like throughout (operands of the matrix instructions are split
  * in two halves). After an eviction positions count the kept tokens.
  * wsum (NULL: none) [nseq][Hkv][cap] fp32: every visible key's softmax weights, summed over the T tokens and the
- * H / Hkv heads of its kv head, are added to its entry. The first call with a larger problem grows the context's
- * workspace (make one before capturing a CUDA graph); calls on one context run one after another. */
+ * H / Hkv heads of its kv head, are added to its entry. */
 typedef struct ork_b200_kv4_attn {
   const void *q;
   void *out;
@@ -217,7 +218,7 @@ int ork_b200_kv4_attn_async(ork_npu *ctx, const ork_b200_kv4 *c, const ork_b200_
  * slots 0.. of dst[i] [nseq][Hkv][dcap], dcap >= keep: the planes of a 4-bit cache, or of an fp32 one. No source
  * overlaps a destination. kept [nseq][Hkv][keep]: the source slots (-1 past the kept ones); score_out
  * [nseq][Hkv][dcap]: their scores (0 up to `keep`), ready to accumulate on; len_out [nseq]: min(n, keep); it may be
- * len itself. kept, score_out and len_out may be NULL. max_len: the largest n. The workspace as in ork_b200_kv4_attn_async. */
+ * len itself. kept, score_out and len_out may be NULL. max_len: the largest n. */
 #define ORK_B200_EVICT_PLANES 8
 typedef struct ork_b200_evict {
   const float *score;

@@ -122,11 +122,42 @@ bool grow(void **p, size_t *cap, size_t need) {
   return true;
 }
 
-unsigned int *zeroed_counts(ork_npu *c, size_t n) {
-  const size_t had = c->capK;
-  if (!grow(&c->dK, &c->capK, (kAttnCounts + n) * sizeof(unsigned int))) return nullptr;
-  if (c->capK != had && cudaMemsetAsync(c->dK, 0, c->capK, c->stream) != cudaSuccess) return nullptr;
-  return (unsigned int *)c->dK;
+bool work_block(ork_npu *c, const char *name, Block *b, size_t need) {
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  const bool capturing = cudaStreamIsCapturing(c->stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone;
+  if (b->cap < need) {
+    if (capturing) {
+      cudaGetLastError();
+      fprintf(stderr, "[ork] ERROR %s: the workspace would grow during CUDA-graph capture; make one call of this size "
+                      "before capturing\n", name);
+      return false;
+    }
+    if (b->graphed) {  // replays of the graph go on using it
+      c->outgrown.push_back(b->p);
+      c->capO += b->cap;
+      *b = Block();
+    }
+    if (!grow(&b->p, &b->cap, need)) {
+      cudaGetLastError();
+      fprintf(stderr, "[ork] ERROR %s: out of device memory\n", name);
+      return false;
+    }
+  }
+  b->graphed = b->graphed || capturing;
+  return true;
+}
+
+unsigned int *zeroed_counts(ork_npu *c, const char *name, size_t n) {
+  const void *had = c->counts.p;
+  const size_t cap = c->counts.cap;
+  if (!work_block(c, name, &c->counts, (kAttnCounts + n) * sizeof(unsigned int))) return nullptr;
+  if (c->counts.p == had && c->counts.cap == cap) return (unsigned int *)c->counts.p;
+  const cudaError_t e = cudaMemsetAsync(c->counts.p, 0, c->counts.cap, c->stream);
+  if (e == cudaSuccess) return (unsigned int *)c->counts.p;
+  log_err(name, e);
+  cudaFree(c->counts.p);  // not handed out: what it holds is not zero
+  c->counts = Block();
+  return nullptr;
 }
 
 bool overlaps(const void *a, size_t an, const void *b, size_t bn) {
@@ -427,8 +458,9 @@ void ork_npu_free(ork_npu *c) {
     layer_tabs_free(c);
     if (c->dL) cudaFree(c->dL);
     if (c->dX) cudaFree(c->dX);
-    if (c->dW) cudaFree(c->dW);
-    if (c->dK) cudaFree(c->dK);
+    if (c->work.p) cudaFree(c->work.p);
+    if (c->counts.p) cudaFree(c->counts.p);
+    for (void *p : c->outgrown) cudaFree(p);
     if (c->dG) cudaFree(c->dG);
     if (c->dF) cudaFree(c->dF);
     if (c->hP) cudaFreeHost(c->hP);
@@ -621,7 +653,7 @@ int ork_b200_f16_mm_run_async(ork_npu *c, ork_w *w, int M, const ork_f16 *dA, fl
 }
 
 size_t ork_b200_staging_bytes(const ork_npu *c) {
-  return c ? c->capA + c->capC + c->capS + c->capL + c->capX + c->capP + c->capW + c->capK : 0;
+  return c ? c->capA + c->capC + c->capS + c->capL + c->capX + c->capP + c->work.cap + c->counts.cap + c->capO : 0;
 }
 
 int ork_b200_reload_tuning(ork_npu *c) {

@@ -591,8 +591,8 @@ extern "C" int ork_b200_attn_async(ork_npu *c, const ork_b200_attn *a) {
   ork_b200_attn d = *a;
   d.window = d.window < d.max_k ? d.window : 0;  // a window over everything is none
   d.sinks = std::min(d.sinks, d.max_k);
-  unsigned int *count = zeroed_counts(c, 0);
-  if (!count) return refuse("out of device memory");
+  unsigned int *count = zeroed_counts(c, "ork_b200_attn_async", 0);
+  if (!count) return -1;
   const bool f16 = d.type == ORK_B200_F16, wide = d.dk == 128;
   const cudaError_t e = f16 ? (wide ? launch_attn<__half, 128>(d, count, c->stream) : launch_attn<__half, 64>(d, count, c->stream))
                             : (wide ? launch_attn<__nv_bfloat16, 128>(d, count, c->stream)

@@ -327,9 +327,9 @@ extern "C" int ork_b200_evict_async(ork_npu *c, const ork_b200_evict *e) {
     if (!device_ptrs_ok(c, "ork_b200_evict_async", {e->src[p], e->dst[p]})) return -1;
   const int chunks = (e->max_len + kChunk - 1) / kChunk, cover = (std::max(e->max_len, e->keep) + kChunk - 1) / kChunk;
   const size_t pb = (rows * sizeof(Picked) + 255) / 256 * 256;
-  if (!grow(&c->dW, &c->capW, pb + rows * std::max(chunks, 1) * sizeof(int2))) return refuse("out of device memory");
-  Picked *picked = (Picked *)c->dW;
-  int2 *before = (int2 *)((uint8_t *)c->dW + pb);
+  if (!work_block(c, "ork_b200_evict_async", &c->work, pb + rows * std::max(chunks, 1) * sizeof(int2))) return -1;
+  Picked *picked = (Picked *)c->work.p;
+  int2 *before = (int2 *)((uint8_t *)c->work.p + pb);
   ork_b200_evict d = *e;
   // CTAs a (sequence, head): about two waves of the SMs in all, 4096 tokens each or more
   int size = 1;

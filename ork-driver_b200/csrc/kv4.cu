@@ -1234,13 +1234,13 @@ int ork_b200_kv4_attn_async(ork_npu *c, const ork_b200_kv4 *kv, const ork_b200_k
   const size_t prows = (size_t)k.nseq * k.Hkv * k.prow, parts = k.splits > 1 ? prows * k.splits : 0;
   const size_t mlb = whole(parts * sizeof(float2)), pob = whole(parts * kv->dk * 4), stb = a->wsum ? whole(prows * 4) : 0;
   const size_t need = mlb + pob + stb + (a->wsum ? prows * k.vis * 4 : 0);
-  if (need && !grow(&c->dW, &c->capW, need)) return refuse(name, "out of device memory");
+  if (need && !work_block(c, name, &c->work, need)) return -1;
   if (k.join || (a->wsum && k.splits > 1)) {
-    unsigned int *z = zeroed_counts(c, (size_t)k.nseq * k.Hkv * k.tiles);
-    if (!z) return refuse(name, "out of device memory");
+    unsigned int *z = zeroed_counts(c, name, (size_t)k.nseq * k.Hkv * k.tiles);
+    if (!z) return -1;
     k.done = z + kAttnCounts;
   }
-  uint8_t *ws = (uint8_t *)c->dW;
+  uint8_t *ws = (uint8_t *)c->work.p;
   k.pml = (float2 *)ws, k.po = (float *)(ws + mlb), k.stat = (float *)(ws + mlb + pob), k.x = (float *)(ws + mlb + pob + stb);
   const cudaError_t e = with_elem(a->type, [&](auto *t) {
     using E = std::remove_pointer_t<decltype(t)>;

@@ -7,9 +7,19 @@
 #include <stdint.h>
 
 #include <initializer_list>
+#include <vector>
 
 #include "ork_internal.h"
 #include "ork_b200.h"
+
+namespace orkb {
+// A device block that grows on demand and that captured CUDA graphs may point to (work_block).
+struct Block {
+  void *p = nullptr;
+  size_t cap = 0;
+  bool graphed = false;  // a captured call was given it
+};
+}  // namespace orkb
 
 struct ork_npu {
   int device = 0;
@@ -26,10 +36,10 @@ struct ork_npu {
   size_t capL = 0;
   void *dX = nullptr;    // the residual stream between multi-launch layers (layer.cu)
   size_t capX = 0;
-  void *dW = nullptr;    // workspace of the long-context operators (kv4.cu, evict.cu)
-  size_t capW = 0;
-  void *dK = nullptr;    // counters of the long-context operators, zero between launches (zeroed_counts)
-  size_t capK = 0;
+  orkb::Block work;      // workspace of the long-context operators (kv4.cu, evict.cu)
+  orkb::Block counts;    // counters of the long-context operators, zero between launches (zeroed_counts)
+  std::vector<void *> outgrown;  // blocks that captured graphs may still use, kept until the context is freed
+  size_t capO = 0;
   void *ltabs = nullptr; // device tables of persistent-layer pointer lists (layer.cu)
   void *dG = nullptr;    // 16 bytes, zero between calls: the argmax's running key and CTA count (decode_glue.cu)
   unsigned int *dF = nullptr;  // tensor-core split-K tile flags, orkb::kTcFlagTiles x 2 words, zero between launches
@@ -87,10 +97,14 @@ bool device_ptrs_ok(const ork_npu *c, const char *name, std::initializer_list<co
 // on the context is refused meanwhile (message + true), the reference's one-job-in-flight contract
 // (include/ork/chain.h:126-133) made a checked error.
 bool async_in_flight(const ork_npu *c, const char *name);
+// Grows one of the context's blocks to at least `need` bytes for the call `name`; false with a message and the block as
+// it was, or empty, where there is no memory, and where the stream is being captured (the allocation cannot be). A block
+// that an earlier captured call was given is kept, outgrown, for the graph's replays.
+bool work_block(ork_npu *c, const char *name, Block *b, size_t need);
 // Device counters that are zero, and that every launch leaves zero: kAttnCounts for attn.cu, then n for kv4.cu;
-// nullptr without memory.
+// nullptr as work_block.
 constexpr size_t kAttnCounts = 4;
-unsigned int *zeroed_counts(ork_npu *c, size_t n);
+unsigned int *zeroed_counts(ork_npu *c, const char *name, size_t n);
 bool overlaps(const void *a, size_t an, const void *b, size_t bn);
 // Enqueues one decode layer on device pointers (layer.cu); W = {q, k, v, o, gate, up, down}.
 int layer_enqueue(ork_npu *c, const struct ork_layer_dims *d, ork_w *const *W, const float *attn_norm,

@@ -32,3 +32,58 @@ def test_evict_updates_lengths_in_place(on, nseq, Hkv, n, keep):
         for h in range(Hkv):
             at = evict_want(sc[s, h], m, keep, 2, 5)
             assert kept[s, h].tolist() == at + [-1] * (keep - len(at)), (s, h)
+
+
+# ---- CUDA graphs and the workspace --------------------------------------------------------------------------------
+
+def cache(nseq, Hkv, dk, cap, seed):
+    from test_gpu_longctx import Cache
+
+    c = Cache(nseq, Hkv, dk, cap)
+    for s in range(nseq):
+        c.put(s, rnd((cap, Hkv, dk), seed + 2 * s), rnd((cap, Hkv, dk), seed + 2 * s + 1))
+    return c
+
+
+def kv4_args(q, out, ln, n, wsum=None, typ="f32", scale=None, window=0, sinks=0):
+    return B.KV4Attn(q=q.data_ptr(), out=out.data_ptr(), type=B.TYPES[typ], H=q.shape[2], T=q.shape[1], q_ts=q.stride(1),
+                     q_hs=q.stride(2), len=ln.data_ptr(), max_len=n, scale=scale or q.shape[3] ** -0.5, window=window,
+                     sinks=sinks, wsum=None if wsum is None else wsum.data_ptr())
+
+
+def test_a_graph_replays_after_larger_calls(on):
+    # the graph's workspace and counters stay its own when a later call needs more
+    with B.Context() as own:
+        st = torch.cuda.Stream()
+        own.L.ork_b200_set_stream(own.ctx, st.cuda_stream)
+        n, big = 2000, 60000
+        c, d = cache(1, 2, 64, 2048, 410), cache(1, 2, 64, 60032, 412)
+        q, out, want = rnd((1, 1, 8, 64), 414), torch.zeros((1, 1, 8, 64), device="cuda"), torch.zeros((1, 1, 8, 64), device="cuda")
+        q2, out2, ws2 = rnd((1, 64, 8, 64), 415), torch.zeros((1, 64, 8, 64), device="cuda"), torch.zeros((1, 2, 60032), device="cuda")
+        ws, ln, ln2 = torch.zeros((1, 2, 2048), device="cuda"), ints([n]), ints([big])
+        torch.cuda.synchronize()
+        assert own.L.ork_b200_kv4_attn_async(own.ctx, C.byref(c.c), C.byref(kv4_args(q, want, ln, n, ws))) == 0
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            assert own.L.ork_b200_kv4_attn_async(own.ctx, C.byref(c.c), C.byref(kv4_args(q, out, ln, n, ws))) == 0
+            # what would allocate is refused, and the capture goes on
+            assert own.L.ork_b200_kv4_attn_async(own.ctx, C.byref(d.c), C.byref(kv4_args(q2, out2, ln2, big, ws2))) == -1
+        small = own.L.ork_b200_staging_bytes(own.ctx)
+        assert own.L.ork_b200_kv4_attn_async(own.ctx, C.byref(d.c), C.byref(kv4_args(q2, out2, ln2, big, ws2))) == 0
+        torch.cuda.synchronize()
+        large = own.L.ork_b200_staging_bytes(own.ctx)
+        assert large - small >= 64 * 8 * big * 4  # the logits' block is new, the graph's is still held
+        torch.cuda.empty_cache()
+        other = [torch.full((1 << 18,), 7, dtype=torch.int32, device="cuda") for _ in range(64)]
+        for i in range(3):
+            out.zero_()
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        assert all(bool((o == 7).all()) for o in other)
+        assert abs(float(ws.sum()) - 4 * 8) < 1e-3  # one eager call and three replays, a weight of 1 a head
+        assert own.L.ork_b200_kv4_attn_async(own.ctx, C.byref(d.c), C.byref(kv4_args(q2, out2, ln2, big, ws2))) == 0
+        assert own.L.ork_b200_sync(own.ctx) == 0 and own.L.ork_b200_staging_bytes(own.ctx) == large
+        del g
