@@ -137,7 +137,9 @@ bool work_block(ork_npu *c, const char *name, Block *b, size_t need) {
       c->capO += b->cap;
       *b = Block();
     }
-    if (!grow(&b->p, &b->cap, need)) {
+    // half as much again where there is room: a decode loop's need rises every few tokens, and each growth waits for
+    // the device
+    if (!grow(&b->p, &b->cap, need + need / 2) && (cudaGetLastError(), !grow(&b->p, &b->cap, need))) {
       cudaGetLastError();
       fprintf(stderr, "[ork] ERROR %s: out of device memory\n", name);
       return false;

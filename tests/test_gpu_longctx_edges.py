@@ -87,3 +87,18 @@ def test_a_graph_replays_after_larger_calls(on):
         assert own.L.ork_b200_kv4_attn_async(own.ctx, C.byref(d.c), C.byref(kv4_args(q2, out2, ln2, big, ws2))) == 0
         assert own.L.ork_b200_sync(own.ctx) == 0 and own.L.ork_b200_staging_bytes(own.ctx) == large
         del g
+
+
+def test_a_growing_cache_seldom_grows_the_workspace(on):
+    # a decode loop's logits grow with every unit of 16 tokens; the workspace by half at a time: 2 MB of logits at first,
+    # 8 MB at last, four growths
+    with B.Context() as own:
+        own.L.ork_b200_set_stream(own.ctx, 1)
+        c = cache(1, 8, 64, 32768, 420)
+        q, ws, ln = rnd((1, 1, 64, 64), 422), torch.zeros((1, 8, 32768), device="cuda"), ints([100])
+        out, sizes = torch.zeros_like(q), set()
+        for n in range(8192, 32769, 256):
+            assert own.L.ork_b200_kv4_attn_async(own.ctx, C.byref(c.c), C.byref(kv4_args(q, out, ln, n, ws))) == 0
+            sizes.add(own.L.ork_b200_staging_bytes(own.ctx))
+        assert own.L.ork_b200_sync(own.ctx) == 0
+        assert len(sizes) <= 5
