@@ -585,6 +585,7 @@ extern "C" int ork_b200_attn_async(ork_npu *c, const ork_b200_attn *a) {
     if (st < a->dk || st % 8) return refuse("strides are multiples of 8, dk at least");
   if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out) % 16)
     return refuse("q, k, v and out are 16-byte aligned");
+  if (((uintptr_t)a->q_start | (uintptr_t)a->k_start) % 4) return refuse("q_start and k_start are 4-byte aligned");
   DeviceGuard dg(c->device);
   if (!device_ptrs_ok(c, "ork_b200_attn_async", {a->q, a->k, a->v, a->out, a->q_start, a->k_start})) return -1;
   if (a->max_q == 0) return 0;

@@ -307,6 +307,8 @@ extern "C" int ork_b200_evict_async(ork_npu *c, const ork_b200_evict *e) {
   if (!c || !e || !e->score || !e->len) return -1;
   if (e->nseq < 1 || e->Hkv < 1 || (long long)e->nseq * e->Hkv > 65535) return refuse("nseq, Hkv >= 1, their product at most 65535");
   if (e->cap < 1 || e->keep < 1 || e->dcap < e->keep) return refuse("cap, keep >= 1 and dcap >= keep");
+  if (((uintptr_t)e->score | (uintptr_t)e->len | (uintptr_t)e->kept | (uintptr_t)e->score_out | (uintptr_t)e->len_out) % 4)
+    return refuse("score, len, kept, score_out and len_out are 4-byte aligned");
   if (e->max_len < 0 || e->max_len > e->cap) return refuse("max_len is 0 .. cap");
   if (e->sinks < 0 || e->recent < 0 || (long long)e->sinks + e->recent > e->keep) return refuse("sinks + recent is 0 .. keep");
   if (e->nplanes < 0 || e->nplanes > ORK_B200_EVICT_PLANES) return refuse("too many planes");

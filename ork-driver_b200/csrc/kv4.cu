@@ -1151,6 +1151,7 @@ static int kv4_rows(ork_npu *c, const ork_b200_kv4 *kv, const void *k, const voi
   if (ts < kv->dk || hs < kv->dk) return refuse(name, "a row stride below dk");
   const size_t es = elem_bytes(type);
   if (((uintptr_t)k | (uintptr_t)v) % es) return refuse(name, "rows are aligned to their type");
+  if (((uintptr_t)start | (uintptr_t)pos) % 4) return refuse(name, "start and pos are 4-byte aligned");
   DeviceGuard dg(c->device);
   if (!device_ptrs_ok(c, name, {kv->k, kv->v, kv->kp, kv->vp, k, v, start, pos})) return -1;
   if (rows == 0) return 0;
@@ -1207,6 +1208,7 @@ int ork_b200_kv4_attn_async(ork_npu *c, const ork_b200_kv4 *kv, const ork_b200_k
   if (a->max_len < 0 || a->max_len > kv->cap) return refuse(name, "max_len is 0 .. cap");
   if (a->window < 0 || a->sinks < 0) return refuse(name, "window and sinks are not negative");
   if (((uintptr_t)a->q | (uintptr_t)a->out) % elem_bytes(a->type)) return refuse(name, "rows are aligned to their type");
+  if (((uintptr_t)a->len | (uintptr_t)a->wsum) % 4) return refuse(name, "len and wsum are 4-byte aligned");
   DeviceGuard dg(c->device);
   if (!device_ptrs_ok(c, name, {kv->k, kv->v, kv->kp, kv->vp, a->q, a->out, a->len, a->wsum})) return -1;
   if (a->max_len == 0) {

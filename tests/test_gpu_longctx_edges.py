@@ -102,3 +102,35 @@ def test_a_growing_cache_seldom_grows_the_workspace(on):
             sizes.add(own.L.ork_b200_staging_bytes(own.ctx))
         assert own.L.ork_b200_sync(own.ctx) == 0
         assert len(sizes) <= 5
+
+
+# ---- refusals ----------------------------------------------------------------------------------------------------
+
+def test_misaligned_arrays_are_refused(on):
+    i, f = ints([0] * 64), torch.zeros(64 * 64, device="cuda")
+    h = torch.zeros(64 * 64, dtype=torch.float16, device="cuda")
+    c = B.KV4(k=f.data_ptr(), v=f.data_ptr(), kp=h.data_ptr(), vp=h.data_ptr(), nseq=1, Hkv=1, dk=64, cap=64)
+    n = on.launches()
+    for off in (1, 2):
+        ip, fp = i.data_ptr(), f.data_ptr()
+        for bad in (dict(q_start=ip + off), dict(k_start=ip + off)):
+            a = B.Attn(q=h.data_ptr(), k=h.data_ptr(), v=h.data_ptr(), out=h.data_ptr(), type=1, nseq=1, H=1, Hkv=1, dk=64, q_ts=64,
+                       q_hs=64, k_ts=64, k_hs=64, v_ts=64, v_hs=64, o_ts=64, o_hs=64, q_start=ip, k_start=ip, q_rows=1, k_rows=1,
+                       max_q=1, max_k=1, scale=1.0)
+            for k, x in bad.items():
+                setattr(a, k, x)
+            assert on.L.ork_b200_attn_async(on.ctx, C.byref(a)) == -1, bad
+        for start, pos in ((ip + off, None), (None, ip + off)):
+            for call in (on.L.ork_b200_kv4_store_async, on.L.ork_b200_kv4_load_async):
+                assert call(on.ctx, C.byref(c), fp, fp, 0, 1, 64, 64, start, pos) == -1
+        for bad in (dict(len=ip + off), dict(wsum=fp + off)):
+            a = B.KV4Attn(q=fp, out=fp, type=0, H=1, T=1, q_ts=64, q_hs=64, len=ip, max_len=64, scale=1.0)
+            for k, x in bad.items():
+                setattr(a, k, x)
+            assert on.L.ork_b200_kv4_attn_async(on.ctx, C.byref(c), C.byref(a)) == -1, bad
+        for bad in (dict(score=fp + off), dict(len=ip + off), dict(kept=ip + off), dict(score_out=fp + 256 + off), dict(len_out=ip + off)):
+            e = B.Evict(score=fp, len=ip, nseq=1, Hkv=1, cap=64, dcap=8, max_len=64, keep=8, nplanes=0)
+            for k, x in bad.items():
+                setattr(e, k, x)
+            assert on.L.ork_b200_evict_async(on.ctx, C.byref(e)) == -1, bad
+    assert on.launches() == n
