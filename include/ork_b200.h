@@ -184,7 +184,7 @@ typedef struct ork_b200_kv4 {
  * The store, per 64 dims with lowest lo and largest hi, in fp32: step = f16(min((hi - lo) * (1/15), 65504)),
  * lowest = f16(lo) saturated, code = clamp(rint((x - lowest) / step), 0, 15), 0 where the step is 0. Dims that hold
  * a NaN or an infinity give a NaN step and lowest value: the token reads back as NaN wherever it is visible.
- * A slot outside [0, cap) is not written (read) and reported. */
+ * A slot outside [0, cap) is not written (read) and reported; so is a sequence whose offsets decrease or are negative. */
 int ork_b200_kv4_store_async(ork_npu *ctx, const ork_b200_kv4 *c, const void *k, const void *v, int type, int rows,
                              long long ts, long long hs, const int *start, const int *pos);
 int ork_b200_kv4_load_async(ork_npu *ctx, const ork_b200_kv4 *c, void *k, void *v, int type, int rows, long long ts,

@@ -147,6 +147,10 @@ __global__ void __launch_bounds__(kRowThreads, STORE ? 4 : 1) kv4_rows_kernel(Ro
   const int at = threadIdx.x % LANES, w = at * NW % WORDS;
   const bool is_v = at * NW >= WORDS;
   if (t0 >= step) return;  // whole teams; a group's threads stay together
+  if (n < 0 || row0 < 0) {  // offsets that decrease, or begin before the rows
+    if (at == 0) kv4_error();
+    return;
+  }
   // the rows whose slots the cache has
   const long long first = slot0 < 0 ? -(long long)slot0 : 0, end = (long long)r.cap - slot0;
   const int last = (int)max(0LL, min((long long)n, end));

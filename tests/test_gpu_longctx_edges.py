@@ -134,3 +134,25 @@ def test_misaligned_arrays_are_refused(on):
                 setattr(e, k, x)
             assert on.L.ork_b200_evict_async(on.ctx, C.byref(e)) == -1, bad
     assert on.launches() == n
+
+
+# ---- rows into the cache and back --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("start", [[0, 3, 2, 4], [-2, 1, 2, 4]])
+def test_store_offsets_that_decrease_or_are_negative_are_reported(on, start):
+    from test_gpu_longctx import Cache
+
+    x = rnd((4, 1, 64), 430)
+    c = Cache(3, 1, 64, 64, 0, 0.0)
+    st = ints(start)
+    args = (0, 4, 64, 64, st.data_ptr(), None)
+    assert on.L.ork_b200_kv4_store_async(on.ctx, C.byref(c.c), x.data_ptr(), x.data_ptr(), *args) == 0
+    assert on.L.ork_b200_sync(on.ctx) == -1 and on.L.ork_b200_sync(on.ctx) == 0
+    want = Cache(3, 1, 64, 64, 0, 0.0)
+    for s in range(3):
+        if 0 <= start[s] <= start[s + 1]:
+            want.put(s, x[start[s]:start[s + 1]], x[start[s]:start[s + 1]])
+    assert torch.equal(c.k, want.k) and torch.equal(c.kp, want.kp) and torch.equal(c.v, want.v)
+    y = torch.full_like(x, 5.0)
+    assert on.L.ork_b200_kv4_load_async(on.ctx, C.byref(c.c), y.data_ptr(), y.data_ptr(), *args) == 0
+    assert on.L.ork_b200_sync(on.ctx) == -1 and on.L.ork_b200_sync(on.ctx) == 0
