@@ -15,7 +15,9 @@
 // The running maximum follows only when it rises by more than 2^8, so that O is seldom scaled; weights stay below 256.
 // Masks are applied to the tiles that hold an edge; tiles that no row sees are not visited.
 // A value of V that is not finite reaches rows that do not see it (0 * inf): a row whose result is not finite is
-// computed again, from its visible keys alone, by its warp. Rows of V past the sequence are cleared in shared memory.
+// computed again, from its visible keys alone, by its warp, once the CTA has no items left and nobody waits for it (in
+// between, some hundred thousand keys would outlast the bounded waits). Such rows are listed in their own places in out.
+// Rows of V past the sequence are cleared in shared memory.
 //
 // Bound by the chain softmax -> P V -> Q K^T of each tile: a step of two tiles and 128 keys of 128 dims takes 3900
 // clocks, of which the tensor cores work 2050 to 2450 and the exponential unit 2050 (both 56 % active over the launch).
@@ -104,14 +106,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if an
   return d;
 }
 
-// Shared memory: the two Q tiles, the ring, 4 KB for each softmax warp's output, barriers, items.
+// Shared memory: the two Q tiles, the ring, 4 KB for each softmax warp's output, barriers, items, the tensor memory's
+// address, each softmax warp's list of rows to compute again.
 template <int DK>
 struct Smem {
   static constexpr int kSlots = DK == 128 ? 4 : 8;
   static constexpr int kTileBytes = kTile * DK * 2, kChunk = kTile * 128;  // a 64-column block of a tile
   static constexpr int kStage = (2 + kSlots) * kTileBytes, kBar = kStage + 8 * 4096;
   static constexpr int kBars = 2 + 2 * kSlots + 6 + 4, kItem = kBar + kBars * 8;
-  static constexpr int kBytes = 1024 + kItem + 2 * 80 + 16;
+  static constexpr int kList = kItem + 2 * 80 + 16, kBytes = 1024 + kList + 8 * 16;
 };
 static_assert(Smem<128>::kBytes <= 232448 && Smem<64>::kBytes <= 232448, "shared memory");
 
@@ -131,27 +134,105 @@ __device__ __forceinline__ Steps steps_of(int p0, int p1, int window, int sinks)
   return s;
 }
 
-// One row from its visible keys alone, by a warp: lane l holds dims l + 32 u.
+// 16 bytes of a row as fp32
+template <class E>
+__device__ __forceinline__ void widen8(const uint4 &w, float (&x)[8]) {
+  const E *e = reinterpret_cast<const E *>(&w);
+#pragma unroll
+  for (int i = 0; i < 8; i++) x[i] = to_f32(e[i]);
+}
+
+// Rows computed from their visible keys alone, by a warp, kAgain of them over the same keys: 32 keys at a time, a lane's
+// own in the first product, its DK / 32 dims in the second. Row r has its query at q[r], its output at out[r] and the
+// position p[r] (-1: no row); qs: room for their queries in shared memory. Where every row sees one infinite value, 16384
+// tokens of 16 heads of 128 take 93 ms instead of 0.9; a row at a time 260 ms, eight rows 82.
+constexpr int kAgain = 4;
 template <class E, int DK>
-__device__ __forceinline__ void slow_row(const ork_b200_attn &a, const Seq &s, int tok, int h) {
+__device__ __forceinline__ void exact_rows(const ork_b200_attn &a, const Seq &s, int kvh, const E *const (&q)[kAgain],
+                                           E *const (&out)[kAgain], const int (&p)[kAgain], float *qs) {
   constexpr int PER = DK / 32;
-  const int lane = threadIdx.x & 31, kvh = h / (a.H / a.Hkv), p = s.tk - s.tq + tok;
-  const E *q = (const E *)a.q + (s.q0 + tok) * a.q_ts + h * a.q_hs;
-  E *out = (E *)a.out + (s.q0 + tok) * a.o_ts + h * a.o_hs;
-  float qv[PER], o[PER] = {}, m = -INFINITY, l = 0.0f;
-  for (int u = 0; u < PER; u++) qv[u] = to_f32(q[lane + 32 * u]) * a.scale;
-  for (int j = 0; j <= p; j++) {
-    if (a.window && j <= p - a.window && j >= a.sinks) j = p - a.window + 1;
-    const E *k = (const E *)a.k + (s.k0 + j) * a.k_ts + kvh * a.k_hs, *v = (const E *)a.v + (s.k0 + j) * a.v_ts + kvh * a.v_hs;
-    float x = 0.0f;
-    for (int u = 0; u < PER; u++) x += qv[u] * to_f32(k[lane + 32 * u]);
-    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    const float mn = fmaxf(m, x), c = m == mn ? 1.0f : expf(m - mn), w = expf(x - (mn == -INFINITY ? 0.0f : mn));
-    l = l * c + w;
-    for (int u = 0; u < PER; u++) o[u] = o[u] * c + w * to_f32(v[lane + 32 * u]);
-    m = mn;
+  const int lane = threadIdx.x & 31;
+  int first = 0x7fffffff, last = -1;
+  float o[kAgain][PER], m[kAgain], l[kAgain];
+  __syncwarp();
+#pragma unroll
+  for (int r = 0; r < kAgain; r++) {
+    m[r] = -INFINITY, l[r] = 0.0f;
+    if (p[r] >= 0) first = min(first, p[r]), last = max(last, p[r]);
+#pragma unroll
+    for (int u = 0; u < PER; u++) {
+      o[r][u] = 0.0f;
+      qs[r * DK + PER * lane + u] = p[r] >= 0 ? to_f32(q[r][PER * lane + u]) * a.scale : 0.0f;
+    }
   }
-  for (int u = 0; u < PER; u++) out[lane + 32 * u] = from_f32<E>(l == 0.0f ? 0.0f : o[u] / l);
+  __syncwarp();
+  // what any of them sees: ns sinks, then lo .. last
+  const int lo = a.window ? max(0, first - a.window + 1) : 0, ns = min(a.sinks, lo), n = ns + last + 1 - lo;
+  const uint32_t sq = sm100::smem_addr(qs);
+  const E *kb = (const E *)a.k + s.k0 * a.k_ts + kvh * a.k_hs, *vb = (const E *)a.v + s.k0 * a.v_ts + kvh * a.v_hs + PER * lane;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int i = min(i0 + lane, n - 1), j = i < ns ? i : i - ns + lo;
+    float w[kAgain] = {};
+    uint4 kw[DK / 8];
+#pragma unroll
+    for (int d = 0; d < DK / 8; d++) kw[d] = reinterpret_cast<const uint4 *>(kb + j * a.k_ts)[d];
+#pragma unroll
+    for (int d = 0; d < DK / 8; d++) {
+      float kd[8];
+      widen8<E>(kw[d], kd);
+#pragma unroll
+      for (int r = 0; r < kAgain; r++) {
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+          float4 f;  // read where it is used, there are more than registers hold
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
+                       : "r"(sq + (r * DK + 8 * d + h) * 4)
+                       : "memory");
+          w[r] = fmaf(f.x, kd[h], fmaf(f.y, kd[h + 1], fmaf(f.z, kd[h + 2], fmaf(f.w, kd[h + 3], w[r]))));
+        }
+      }
+    }
+    bool done = true;
+#pragma unroll
+    for (int r = 0; r < kAgain; r++) {
+      const bool see = i0 + lane < n && j <= p[r] && (a.window == 0 || j > p[r] - a.window || j < a.sinks);
+      float mn = see ? w[r] : -INFINITY;
+      for (int d = 16; d; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+      mn = fmaxf(m[r], mn);
+      const float c = m[r] == mn ? 1.0f : expf(m[r] - mn), e = expf(w[r] - (mn == -INFINITY ? 0.0f : mn));
+      float t = see ? e : 0.0f;
+      for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+      l[r] = l[r] * c + t;
+      m[r] = mn;
+#pragma unroll
+      for (int u = 0; u < PER; u++) o[r][u] *= c;
+      w[r] = see ? e : -1.0f;  // no weight: what the row does not see must not reach it
+      done = done && (p[r] < 0 || l[r] != l[r]);
+    }
+    if (done) break;  // a logit that is a NaN or infinite makes its row NaN whatever follows
+    const int cnt = min(32, n - i0);
+#pragma unroll 8
+    for (int y = 0; y < cnt; y++) {
+      const E *v = vb + __shfl_sync(0xffffffffu, j, y) * a.v_ts;
+      float x[PER];
+#pragma unroll
+      for (int u = 0; u < PER; u++) x[u] = to_f32(v[u]);
+#pragma unroll
+      for (int r = 0; r < kAgain; r++) {
+        const float wy = __shfl_sync(0xffffffffu, w[r], y);
+        if (!(wy < 0.0f))
+#pragma unroll
+          for (int u = 0; u < PER; u++) o[r][u] = fmaf(wy, x[u], o[r][u]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kAgain; r++)
+    if (p[r] >= 0)
+#pragma unroll
+      for (int u = 0; u < PER; u++) out[r][PER * lane + u] = from_f32<E>(l[r] == 0.0f ? 0.0f : o[r][u] / l[r]);
 }
 
 // An item: a head group of a sequence, and a pair of tiles of its tokens.
@@ -160,6 +241,7 @@ struct Item {
   int kvh, h0, tok0, back;  // first head and token; position of token 0
   Steps st[2], all;         // of the tiles, of either
   int end;                  // there are no more items
+  int no;                   // its number
 };
 static_assert(sizeof(Item) <= 80, "an item's place");
 // Items are numbered by tile pair (the last ones first: they see most), then sequence, then head group. False: nothing
@@ -176,6 +258,7 @@ __device__ __forceinline__ bool item_of(const ork_b200_attn &a, int it, int pair
   }
   o->all = steps_of(o->back + o->tok0, o->back + min(o->tok0 + 2 * per, o->s.tq) - 1, a.window, a.sinks);
   o->end = 0;
+  o->no = it;
   return true;
 }
 
@@ -206,6 +289,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     sm100::bar_init_fence();
   }
+  // the items of which the warp has rows to compute again: how many, the latest one's number and first such row. That row
+  // in out holds their bits, and the number and first row of the item before.
+  int4 *again = (int4 *)(smem + M::kList) + (warp & 7);
+  if (warp < 8 && lane == 0) *again = make_int4(0, 0, 0, 0);
   if (warp == 8) sm100::tmem_alloc(sm100::smem_addr(slot), 512);
   sm100::tc_fence_before();
   __syncthreads();
@@ -416,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm100::tmem_ld_wait(x[2]), sm100::tmem_ld_wait(x[3]);
         mask_max(2), mask_max(3);
         const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-        if (!(top < INFINITY)) l = __int_as_float(0x7fc00000);  // an infinity or a NaN among the logits: see slow_row
+        if (!(top < INFINITY)) l = __int_as_float(0x7fc00000);  // an infinity or a NaN among the logits: see exact_rows
         const bool rise = (top - m) * sc > kRise;
         if (__any_sync(0xffffffffu, rise)) {
           const float k2 = rise ? sm100::ex2((m - top) * sc) : 1.0f;
@@ -455,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       bool fin = true;
       const Seq seq = {sm100::uniform(pl->s.q0), sm100::uniform(pl->s.tq), sm100::uniform(pl->s.k0), sm100::uniform(pl->s.tk)};
-      const int h0 = sm100::uniform(pl->h0);
+      const int h0 = sm100::uniform(pl->h0), no = sm100::uniform(pl->no);
       __syncwarp();
       if (lane == 0) sm100::bar_arrive(iempty + 8 * (k & 1));
       E *const base = (E *)a.out + (long long)seq.q0 * a.o_ts + 8 * (lane & 7);
@@ -495,9 +582,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
       const int tok = tok0 + (row >> lp), h = h0 + (row & ((1 << lp) - 1));
-      for (unsigned bad = __ballot_sync(0xffffffffu, tok < seq.tq && !fin); bad; bad &= bad - 1) {
-        const int from = __ffs(bad) - 1;
-        slow_row<E, DK>(a, seq, __shfl_sync(0xffffffffu, tok, from), __shfl_sync(0xffffffffu, h, from));
+      const unsigned bad = __ballot_sync(0xffffffffu, tok < seq.tq && !fin);
+      if (bad && lane == __ffs(bad) - 1) {
+        const int4 e = *again;
+        *(int4 *)((E *)a.out + (long long)(seq.q0 + tok) * a.o_ts + (long long)h * a.o_hs) = make_int4((int)bad, e.y, e.z, 0);
+        *again = make_int4(e.x + 1, no, lane, 0);
+      }
+    }
+    __syncwarp();
+    // whatever out may hold by now (rows that a caller laid over one another), every item and row is checked
+    int4 e = *again;
+    for (int left = ok ? e.x : 0; left && (unsigned)e.y < (unsigned)items && item_of(a, e.y, pairs, lp, groups, &w); left--) {
+      auto token = [&](int rr) { return w.tok0 + t * per + ((wrow + rr) >> lp); };
+      auto place_of = [&](int rr, long long ts, long long hs) {
+        return (long long)(w.s.q0 + token(rr)) * ts + (long long)(w.h0 + ((wrow + rr) & ((1 << lp) - 1))) * hs;
+      };
+      if (token(e.z & 31) >= w.s.tq) break;
+      e = *(const int4 *)((const E *)a.out + place_of(e.z & 31, a.o_ts, a.o_hs));
+      for (unsigned bad = (unsigned)e.x; bad;) {
+        const E *q[kAgain];
+        E *out[kAgain];
+        int p[kAgain];
+#pragma unroll
+        for (int r = 0; r < kAgain; r++) {
+          const int rr = bad ? __ffs(bad) - 1 : 0;
+          p[r] = bad && token(rr) < w.s.tq ? w.back + token(rr) : -1;
+          q[r] = (const E *)a.q + place_of(rr, a.q_ts, a.q_hs), out[r] = (E *)a.out + place_of(rr, a.o_ts, a.o_hs);
+          bad &= bad - 1;
+        }
+        exact_rows<E, DK>(a, w.s, w.kvh, q, out, p, (float *)(smem + M::kStage + warp * 4096));
       }
     }
     if (!ok && lane == 0) attn_failed();

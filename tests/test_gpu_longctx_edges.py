@@ -156,3 +156,61 @@ def test_store_offsets_that_decrease_or_are_negative_are_reported(on, start):
     y = torch.full_like(x, 5.0)
     assert on.L.ork_b200_kv4_load_async(on.ctx, C.byref(c.c), y.data_ptr(), y.data_ptr(), *args) == 0
     assert on.L.ork_b200_sync(on.ctx) == -1 and on.L.ork_b200_sync(on.ctx) == 0
+
+
+# ---- prompt attention --------------------------------------------------------------------------------------------
+
+def prompt(on, q, k, v, tq, tk, typ, window=0, sinks=0, scale=None):
+    from test_gpu_longctx import attn_call
+
+    out = torch.full_like(q, 9.0)
+    a, held = attn_call(q, k, v, out, tq, tk, typ, window, sinks, scale)
+    assert on.L.ork_b200_attn_async(on.ctx, C.byref(a)) == 0 and on.L.ork_b200_sync(on.ctx) == 0
+    return out
+
+
+def same_but_rounding(got, want, typ, top):
+    # a row's weights are within u / 2 each, its output within u / 2 of itself: u max |v| covers both; NaNs and infinities
+    # lie where they belong
+    u, got = {"f16": 2.0 ** -10, "bf16": 2.0 ** -7}[typ], got.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+    fin = torch.isfinite(want)
+    assert torch.equal(got[~fin].nan_to_num(nan=5.0), want[~fin].nan_to_num(nan=5.0))
+    assert float((got - want)[fin].abs().max()) <= 1.5 * u * top + 2.0 ** -14
+
+
+def test_attn_an_infinite_value_that_every_row_sees(on):
+    # 256 rows after a prefix of 150000 keys, one early value infinite: every row is computed again, which may take its
+    # time, and the other sequence is whole
+    tq, tk, dk = [256, 300], [150000, 300], 128
+    q, k, v = (rnd((sum(n), 1, dk), 440 + i, 1, torch.float16) for i, n in enumerate((tq, tk, tk)))
+    v[7, 0, 5] = math.inf
+    out = prompt(on, q, k, v, tq, tk, "f16")
+    fin = v.clone()
+    fin[7, 0, 5] = 0
+    for i, (q0, k0) in enumerate(((0, 0), (256, 150000))):
+        want, _, _, top = ref.attention(q[q0:q0 + tq[i]], k[k0:k0 + tk[i]], fin[k0:k0 + tk[i]], dk ** -0.5, 0, 0)
+        if i == 0:
+            want[:, 0, 5] = math.inf
+        same_but_rounding(out[q0:q0 + tq[i]], want, "f16", top)
+
+
+@pytest.mark.parametrize("typ,dk,H,Hkv,window,sinks", [("f16", 64, 16, 8, 0, 0), ("bf16", 128, 12, 4, 700, 3)])
+def test_attn_nonfinite_values_in_many_items(on, typ, dk, H, Hkv, window, sinks):
+    # more items than CTAs, most of them with rows that are computed again
+    T = 3000
+    q, k, v = (rnd((T, h, dk), 444 + i, 1, {"f16": torch.float16, "bf16": torch.bfloat16}[typ]) for i, h in enumerate((H, Hkv, Hkv)))
+    fin = v.clone()
+    hit = {}
+    for g in range(Hkv):
+        hit[g] = [(1, 3, math.inf), (90 + 130 * g, dk - 1, math.nan), (2500, 17, -math.inf)]
+        for j, d, x in hit[g]:
+            v[j, g, d], fin[j, g, d] = x, 0
+    out = prompt(on, q, k, v, [T], [T], typ, window, sinks)
+    want, _, _, top = ref.attention(q, k, fin, dk ** -0.5, window, sinks)
+    ok = ref.mask(T, T, window, sinks, q.device)
+    for g in range(Hkv):
+        for j, d, x in hit[g]:
+            for h in range(g * (H // Hkv), (g + 1) * (H // Hkv)):
+                want[ok[:, j], h, d] = x
+    same_but_rounding(out, want, typ, top)
