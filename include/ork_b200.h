@@ -151,8 +151,9 @@ int ork_b200_argmax_scaled_async(ork_npu *ctx, const int32_t *C, const float *bs
  * of the last `window` keys, the first `sinks` keys staying visible. out = sum over the visible keys of
  * softmax(scale * q . k) v; a row that sees no key (p < 0) gives zeros. Rows of all sequences are packed; row r of
  * head h lies at q + r * q_ts + h * q_hs, its dk values contiguous, likewise k, v and out.
- * type ORK_B200_F16 or ORK_B200_BF16 (inputs and output); scale is positive; the scores and the output are summed in fp32 and the
- * softmax weights enter the second product rounded to `type`. Bases are 16-byte aligned, strides multiples of 8.
+ * type ORK_B200_F16 or ORK_B200_BF16 (inputs and output); scale is positive; the scores and the output are summed in
+ * fp32 and the softmax weights enter the second product rounded to `type` (fp16: to 2^-32 of the row's largest at best).
+ * Bases are 16-byte aligned, strides multiples of 8.
  * out overlaps no input. q_start, k_start: device int [nseq + 1]; q_rows / k_rows: rows that q and out / k and v
  * hold; max_q / max_k: the most rows of any one sequence (they size the launch). */
 typedef struct ork_b200_attn {

@@ -4,7 +4,7 @@
 // One CTA per SM takes items, two tiles of 128 query rows of one kv head, and streams the keys that any of them sees, 128
 // at a time; the loads and products of an item begin under the end of the one before:
 //   S = Q K^T     128 x 128 x dk, both operands in shared memory, S in tensor memory (fp32)
-//   P = 2^(S sc - m)  online softmax, a thread per row; P goes back to tensor memory in 16 bits, over S
+//   P = 2^(S sc - m + top)  online softmax, a thread per row; P goes back to tensor memory in 16 bits, over S
 //   O += P V      128 x dk x 128, P from tensor memory, V in shared memory as it lies (N-major), O in tensor memory
 // The two tiles alternate: while one is in its softmax the tensor cores work for the other. A row of a tile is a
 // (token, head) pair, `pack` heads of the group (its largest power of two, at most 8) side by side, so that few tokens
@@ -12,7 +12,8 @@
 // Roles (three warpgroups): 0 and 1 the softmax and output of tile 0 and 1; of the third, warp 8 issues the products and
 // warp 9 the TMA loads into a ring of 128 x dk slots that K and V tiles share. It gives most of its registers to the
 // others, whose threads hold a row of S each.
-// The running maximum follows only when it rises by more than 2^8, so that O is seldom scaled; weights stay below 256.
+// The running maximum follows only when it rises by more than 2^8, so that O is seldom scaled; weights stay below 2^8 (fp16:
+// 2^15, kTop).
 // Masks are applied to the tiles that hold an edge; tiles that no row sees are not visited.
 // A value of V that is not finite reaches rows that do not see it (0 * inf): a row whose result is not finite is
 // computed again, from its visible keys alone, by its warp, once the CTA has no items left and nobody waits for it (in
@@ -69,6 +70,10 @@ __device__ __forceinline__ bool seq_of(const ork_b200_attn &a, int s, Seq *o) {
 constexpr int kTile = 128;    // query rows of a tile, keys of a step
 constexpr int kThreads = 384;
 constexpr float kRise = 8.0f;  // log2 of the rise of a maximum that O is scaled for
+// log2 of the weight of the running maximum. With kRise it fills fp16's range to 2^15, so that a weight is lost to the
+// second product below 2^-32 of the maximum's, not 2^-25: 131072 of those would be 0.4 % of a row. bf16 needs none of it.
+template <class E>
+constexpr float kTop = std::is_same<E, __half>::value ? 7.0f : 0.0f;
 
 __device__ __forceinline__ void attn_failed() {
   atomicOr(&g_attn_error, 1u);
@@ -521,7 +526,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float2 mu = m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-m * sc, -m * sc);
+        const float off = m == -INFINITY ? 0.0f : fmaf(-m, sc, kTop<E>);
+        const float2 mu = make_float2(off, off);
 #pragma unroll
         for (int c = 0; c < 4; c++) weights(c, mu);
         l += sum.x + sum.y;

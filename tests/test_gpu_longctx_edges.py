@@ -214,3 +214,25 @@ def test_attn_nonfinite_values_in_many_items(on, typ, dk, H, Hkv, window, sinks)
             for h in range(g * (H // Hkv), (g + 1) * (H // Hkv)):
                 want[ok[:, j], h, d] = x
     same_but_rounding(out, want, typ, top)
+
+
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("first", [True, False])
+def test_attn_a_long_tail_far_below_one_key(on, typ, first):
+    # one key 18 nats above 16384 others, and all of the output theirs: 2^-26 of the weight each, 2^-12 together. The tail
+    # is within its weights' rounding (u / 2 of each; fp16 holds them to 2^-32 of the largest), the output's, and the
+    # logits' error (2^-22 of 18 nats)
+    n, dk, top = 16384, 64, 60.0
+    u = {"f16": 2.0 ** -10, "bf16": 2.0 ** -7}[typ]
+    dt = {"f16": torch.float16, "bf16": torch.bfloat16}[typ]
+    q, k, v = torch.zeros((1, 2, dk), device="cuda", dtype=dt), rnd((n + 1, 1, dk), 460, 1, dt), torch.full((n + 1, 1, dk), top, device="cuda", dtype=dt)
+    q[..., 0], q[..., 1] = 1.0, 0.25
+    k[..., 0] = 0.0
+    at = 0 if first else n - 3
+    k[at, 0, :2] = torch.tensor([18.0, 0.0], device="cuda").to(dt)
+    v[at] = 0.0
+    out = prompt(on, q, k, v, [1], [n + 1], typ, scale=1.0)
+    want, _, _, _ = ref.attention(q, k, v, 1.0, 0, 0)
+    tol = (1.5 * u + 2.0 ** -15) * float(want.max()) + (n * 2.0 ** -32 * top if typ == "f16" else 0.0)
+    assert float(want.min()) > 3 * tol
+    assert float((out.double() - want).abs().max()) <= tol
