@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
     mx = quad_max(mx);
     const unsigned quad = 15u << (lane & 28);
     fin = (__ballot_sync(0xffffffffu, fin) & quad) == quad;
-    const int e = fin ? max(-100, min(100, 147 - (int)(__float_as_uint(mx) >> 23))) : 0;
+    const int e = fin ? min(100, 147 - (int)(__float_as_uint(mx) >> 23)) : 0;  // -107 at least
     const float up = pow2(e), f = fin ? a.scale * 1.4426950408889634f * pow2(-e) : __int_as_float(0x7fc00000);
     if (c == 0) qm->f[y * kRows + r] = f;
 #pragma unroll

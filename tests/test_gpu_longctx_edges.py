@@ -236,3 +236,18 @@ def test_attn_a_long_tail_far_below_one_key(on, typ, first):
     tol = (1.5 * u + 2.0 ** -15) * float(want.max()) + (n * 2.0 ** -32 * top if typ == "f16" else 0.0)
     assert float(want.min()) > 3 * tol
     assert float((out.double() - want).abs().max()) <= tol
+
+
+# ---- attention over the 4-bit cache ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("power", [118, 121, 124])
+def test_kv4_attn_queries_near_the_top_of_their_range(on, typ, power):
+    # queries of 2^power and a scale that takes it back: the same logits as those of ordinary queries
+    from test_gpu_longctx import Cache, attn4_check
+
+    c = Cache(1, 2, 64, 320)
+    c.put(0, rnd((300, 2, 64), 470), rnd((300, 2, 64), 471))
+    q = rnd((1, 2, 8, 64), 472, 1.5, {"f32": torch.float32, "bf16": torch.bfloat16}[typ]) * 2.0 ** power
+    assert torch.isfinite(q).all()
+    attn4_check(on, c, q, [300], typ, scale=0.125 * 2.0 ** -power)
