@@ -618,14 +618,21 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
 #pragma unroll
           for (int g = 0; g < NG; g++)
             if (!seen) kf[g] = vf[g] = make_float2(0.0f, 0.0f);
-          // a value that is not a number reaches the rows that see the token through its logit: 0 * NaN would
-          // reach them all
-          bool bad = false;
+          // values that are not numbers reach the rows that see the token by the sums of the lowest values: 0 * NaN
+          // would reach them all
+          const unsigned lanes = kStageTok % 32 == 0 || i + 1 < PT ? 0xffffffffu : (1u << kStageTok % 32) - 1;
 #pragma unroll
-          for (int g = 0; g < NG; g++) bad = bad || !(fabsf(vf[g].x) <= 1e6f) || !(fabsf(vf[g].y) <= 1e6f);
-          if (bad) {
+          for (int g = 0; g < NG; g++) {
+            const bool bad = !(fabsf(vf[g].x) <= 1e6f && fabsf(vf[g].y) <= 1e6f);
+            if (bad) vf[g] = both(0.0f);
+#pragma unroll 1
+            for (unsigned at = __ballot_sync(lanes, bad); at; at &= at - 1)
 #pragma unroll
-            for (int g = 0; g < NG; g++) kf[g] = both(__int_as_float(0x7fc00000)), vf[g] = both(0.0f);
+              for (int y = 0; y < NT; y++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                  if (visible(a, n - a.T + (tile * TR + y * kRows + 2 * c + h) / G, tok0 + 32 * i + __ffs(at) - 1))
+                    z[y][g][h] = __int_as_float(0x7fc00000);
           }
         }
         float kpar[2 * NG];

@@ -251,3 +251,19 @@ def test_kv4_attn_queries_near_the_top_of_their_range(on, typ, power):
     q = rnd((1, 2, 8, 64), 472, 1.5, {"f32": torch.float32, "bf16": torch.bfloat16}[typ]) * 2.0 ** power
     assert torch.isfinite(q).all()
     attn4_check(on, c, q, [300], typ, scale=0.125 * 2.0 ** -power)
+
+
+@pytest.mark.parametrize("T,window", [(1, 0), (3, 0), (3, 50)])
+@pytest.mark.parametrize("token", [10, 60, 97, 98, 99])
+def test_kv4_attn_nan_values_reach_their_own_group_alone(on, T, window, token):
+    # wherever the token lies in what is loaded at once: its 64 dims are NaN in the rows that see it, the other dims and
+    # the weights are the finite ones
+    from test_gpu_longctx import Cache, attn4_check
+
+    c = Cache(1, 2, 128, 128)
+    c.put(0, rnd((100, 2, 128), 480), rnd((100, 2, 128), 481))
+    c.vp[0, 1, token, 1] = math.nan
+    out = attn4_check(on, c, rnd((1, T, 8, 128), 482), [100], "f32", window, 0)
+    assert torch.isfinite(out[..., :4, :]).all() and torch.isfinite(out[..., :64]).all()
+    seen = torch.tensor([token <= 100 - T + t and (not window or token > 100 - T + t - window) for t in range(T)])
+    assert torch.equal(torch.isnan(out[0, :, 4:, 64:]).all(-1).all(-1).cpu(), seen)
