@@ -267,9 +267,17 @@ __global__ void __launch_bounds__(kRowThreads, STORE ? 4 : 1) kv4_rows_kernel(Ro
 // Second product, mma.m16n8k16 of fp16: the output has no more than 11 bits either. A shift and two ANDs put two nibbles
 // of each 16-bit half into the mantissa, as the subnormals code * 2^-22 and code * 2^-18, and the scales are taken out of
 // the sums at the end. (Left where the byte has them, a shift less, 131071 tokens came out off by 6e-4 instead of
-// 2.7e-4.) p * step, rounded to fp16, is transposed between the products with movmatrix; a power of two per warp keeps
-// it in range. For fp32 queries (SPLIT) it is split into an fp16 and the fp16 of what that leaves, 22 bits together, the
-// product runs twice, and every code is shifted to the top of the mantissa, code * 2^-18.
+// 2.7e-4.) p * step, rounded to fp16, is transposed between the products with movmatrix. For fp32 queries (SPLIT) it is
+// split into an fp16 and the fp16 of what that leaves, 22 bits together, the product runs twice, and every code is shifted
+// to the top of the mantissa, code * 2^-18.
+// What keeps p * step in fp16's range: the steps of each group of 64 dims are scaled by a power of two, the one that
+// brings the largest of the warp's first stage to 1 at least and less than 2; and a row's p is 2^(x - m) for an m that
+// follows not the largest logit but the largest p * step, the logit plus the exponent of the token's larger scaled step.
+// So the row's largest p * step lies between 2^(kTop - 6) and 2^15 in one group at least. What is 2^-16 of it, and more,
+// is rounded to 11 bits (what is 2^-5 of it, and more, to 22), and smaller ones to 2^-27 of it: a token of large steps
+// that has no weight costs the others no digits, nor does a group of large steps the other group. With one scale of both
+// groups, by the largest step of the warp's tokens, a group of steps 10^4 times smaller was off by 6e-4 instead of 8e-7
+// (fp32 queries), and 32768 tokens 19 nats below another one by 7e-2 instead of 1e-6.
 // The codes of v are not negative although v has no sign: their sum would grow far above the output that it is to
 // leave after the lowest values' share is added, and the tensor cores truncate what they add. So each stage ends
 // with 8 * sum(p * step) taken out again (the sum by a product with ones, so that it holds the rounded p * step), and
@@ -297,10 +305,15 @@ constexpr int kUnit = 16;   // tokens
 constexpr int kStageUnits = 3;
 constexpr int kStageTok = kUnit * kStageUnits;
 constexpr int kRows = 8;    // query rows of a column tile
-// The sums are scaled by 2^-m for an m that only follows the running maximum once that is kRise above it: most
-// stages raise the maximum of some of the eight rows a little, and scaling the accumulators for that was a fifth of
-// the instructions. Weights reach 2^kRise; times the largest scaled step (64) they stay below fp16's 65504.
-constexpr float kRise = 5.0f;
+// m only follows the running maximum of p * step (log2) once that is kTop + kRise above it, and then to kTop below it:
+// most stages raise the maximum of some of the eight rows a little, and scaling the accumulators for that was a fifth of
+// the instructions.
+constexpr float kTop = 8.0f, kRise = 5.0f;
+// Scaled steps between these count as 1 in the maximum, and nearly all are: a stage of none but those takes the maximum of
+// the logits alone (0.6 % of the time of a full batch went to the test, 7 % to the exact maximum in every stage). With them
+// p * step reaches 2^(kTop + kRise) * 4 = 2^15.
+constexpr float kOddBelow = 0x1p-6f, kOddAbove = 4.0f;
+constexpr int kNoStep = -60;  // log2 of the step that a token of smaller steps counts as, so that p stays finite
 
 struct Attn4 {
   const uint8_t *kc, *vc;
@@ -593,7 +606,10 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
         for (int j = 0; j < 4; j++) o[y][g][j][i] = o[y][g][j][i + 2] = 0.0f;
       }
     }
-  float vs = 1.0f, vlim = 0.0f;  // scale of p * step, and the largest step it is good for (the first stage sets both)
+  float vs[NG];  // scales of the groups' steps; 0 until a stage has any
+  bool unset = true;
+#pragma unroll
+  for (int g = 0; g < NG; g++) vs[g] = 0.0f;
   bool ok = true;
   int slot = 0;
   uint32_t parity = 0;
@@ -605,7 +621,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
     // every token of the stage visible to every row?
     const bool whole = cnt == kStageUnits && tok1 <= n - a.T + 1 && (a.window == 0 || tok0 > n - 1 - a.window || tok1 <= a.sinks);
     constexpr int PT = (kStageTok + 31) / 32;
-    float vpar[PT][2 * NG], top = 0.0f;  // of the tokens that this lane widens
+    float vpar[PT][2 * NG];  // of the tokens that this lane widens
 #pragma unroll
     for (int i = 0; i < PT; i++) {
       const int tk = lane + 32 * i, j = tok0 + tk;
@@ -640,33 +656,46 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
         for (int g = 0; g < NG; g++) {
           kpar[g] = kf[g].x, kpar[NG + g] = kf[g].y;
           vpar[i][g] = vf[g].x, vpar[i][NG + g] = fmaf(8.0f, vf[g].x, vf[g].y);
-          top = fmaxf(top, vf[g].x);
         }
         store_pars(wide->k[tk], kpar);
       }
     }
-    if (__any_sync(0xffffffffu, top > vlim)) {  // rare: steps rarely grow 32-fold
-      for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      // the largest step becomes 1 .. 2
-      const float ns = pow2(min(127 - (int)(__float_as_uint(top) >> 23), 100)), k = vlim > 0.0f ? ns / vs : 0.0f;
-      vs = ns;
-      vlim = 64.0f / ns;
+    if (unset) {
+      unset = false;
 #pragma unroll
-      for (int y = 0; y < NT; y++)
+      for (int g = 0; g < NG; g++)
+        if (vs[g] == 0.0f) {
+          float top = 0.0f;
 #pragma unroll
-        for (int g = 0; g < NG; g++)
-#pragma unroll
-          for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[y][g][j][i] *= k;
+          for (int i = 0; i < PT; i++)
+            if (kStageTok % 32 == 0 || lane + 32 * i < kStageTok) top = fmaxf(top, fabsf(vpar[i][g]));
+          const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+          if (bits && bits < 0x7f800000u) vs[g] = pow2(127 - (int)(bits >> 23));
+          else unset = true;
+        }
     }
+    float top[PT];  // the tokens' larger steps
 #pragma unroll
     for (int i = 0; i < PT; i++) {
       const int tk = lane + 32 * i;
+      top[i] = top[0];
       if (kStageTok % 32 == 0 || tk < kStageTok) {
 #pragma unroll
-        for (int g = 0; g < NG; g++) vpar[i][g] *= vs;
+        for (int g = 0; g < NG; g++) vpar[i][g] *= vs[g];
         store_pars(wide->v[tk], vpar[i]);
+        top[i] = fmaxf(fabsf(vpar[i][0]), fabsf(vpar[i][NG - 1]));
+      }
+    }
+    float most = top[0], least = top[0];
+#pragma unroll
+    for (int i = 1; i < PT; i++) most = fmaxf(most, top[i]), least = fminf(least, top[i]);
+    bool odd = most > kOddAbove || least < kOddBelow;
+    if (!whole) {  // of the tokens that the stage has
+      odd = false;
+#pragma unroll
+      for (int i = 0; i < PT; i++) {
+        const int tk = lane + 32 * i;
+        odd = odd || (tk < cnt * kUnit && tok0 + tk < n && !(top[i] >= kOddBelow && top[i] <= kOddAbove));
       }
     }
     __syncwarp();
@@ -744,21 +773,43 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
     }
     float mx[NT][2];
     bool rise = false;
+    if (!__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+      for (int y = 0; y < NT; y++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          mx[y][i] = fmaxf(x[y][0][i], x[y][0][2 + i]);
+#pragma unroll
+          for (int w = 1; w < kStageUnits; w++) mx[y][i] = fmaxf(mx[y][i], fmaxf(x[y][w][i], x[y][w][2 + i]));
+        }
+    } else {
+#pragma unroll
+      for (int w = 0; w < kStageUnits; w++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          float par[2 * NG];
+          load_pars(wide->v[kUnit * w + 8 * h + mt], par);
+          const int e = (int)(__float_as_uint(fmaxf(fabsf(par[0]), fabsf(par[NG - 1]))) >> 23);
+          const float lt = e < 255 ? (float)max(e - 127, kNoStep) : (float)kNoStep;
+#pragma unroll
+          for (int y = 0; y < NT; y++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const float v = x[y][w][2 * h + i] + lt;
+              mx[y][i] = w + h ? fmaxf(mx[y][i], v) : v;
+            }
+        }
+    }
 #pragma unroll
     for (int y = 0; y < NT; y++)
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        mx[y][i] = fmaxf(x[y][0][i], x[y][0][2 + i]);
-#pragma unroll
-        for (int w = 1; w < kStageUnits; w++) mx[y][i] = fmaxf(mx[y][i], fmaxf(x[y][w][i], x[y][w][2 + i]));
-        rise = rise || mx[y][i] > mrow[y][i] + kRise;
-      }
+      for (int i = 0; i < 2; i++) rise = rise || mx[y][i] > mrow[y][i] + (kTop + kRise);
     if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
       for (int y = 0; y < NT; y++)
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          const float m = fmaxf(mrow[y][i], col_max(mx[y][i])), k = mrow[y][i] == m ? 1.0f : sm100::ex2(mrow[y][i] - m);
+          const float m = fmaxf(mrow[y][i], col_max(mx[y][i]) - kTop), k = mrow[y][i] == m ? 1.0f : sm100::ex2(mrow[y][i] - m);
           mrow[y][i] = m;
           l[y][i] *= k;
 #pragma unroll
@@ -869,7 +920,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   float2 *sml = reinterpret_cast<float2 *>(so + kWarps * TR * LDO);   // [kWarps][TR]
   static_assert(kWarps * TR * (LDO * 4 + 8) + 4 <= kWarps * NST * (int)sizeof(Stage<DK>), "the rings hold it");
   __syncthreads();  // the rings are idle (a warp whose wait gave up has reported it)
-  const float back = (SPLIT ? 0x1p18f : 0x1p22f) / vs, back1 = SPLIT ? back : back * 0.0625f;
+  float back[NG], back1[NG];  // of the even and odd dims of the codes
+#pragma unroll
+  for (int g = 0; g < NG; g++) {
+    back[g] = vs[g] == 0.0f ? 0.0f : (SPLIT ? 0x1p18f : 0x1p22f) / vs[g];
+    back1[g] = SPLIT ? back[g] : back[g] * 0.0625f;
+  }
 #pragma unroll
   for (int y = 0; y < NT; y++)
 #pragma unroll
@@ -883,7 +939,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
         float v[8];
 #pragma unroll
         for (int j = 0; j < 4; j++)
-          v[2 * j] = fmaf(o[y][g][j][i], back, zz), v[2 * j + 1] = fmaf(o[y][g][j][i + 2], back1, zz);
+          v[2 * j] = fmaf(o[y][g][j][i], back[g], zz), v[2 * j + 1] = fmaf(o[y][g][j][i + 2], back1[g], zz);
         float4 *dst = reinterpret_cast<float4 *>(so + rr * LDO + 64 * g + 8 * r);
         dst[0] = make_float4(v[0], v[1], v[2], v[3]);
         dst[1] = make_float4(v[4], v[5], v[6], v[7]);

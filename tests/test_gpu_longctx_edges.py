@@ -267,3 +267,99 @@ def test_kv4_attn_nan_values_reach_their_own_group_alone(on, T, window, token):
     assert torch.isfinite(out[..., :4, :]).all() and torch.isfinite(out[..., :64]).all()
     seen = torch.tensor([token <= 100 - T + t and (not window or token > 100 - T + t - window) for t in range(T)])
     assert torch.equal(torch.isnan(out[0, :, 4:, 64:]).all(-1).all(-1).cpu(), seen)
+
+
+def kv4_error_bound(c, q, n, typ, scale, bits=21):
+    """For one sequence and token, q [H, dk]: what each output may be off by, and the output. Queries enter as integers
+    below 2^bits, a power of two times them, so a logit is off by what that leaves of each dim, times |k|; then by six
+    roundings of fp32 (2^-24 each) of its parts, per group step (q . codes) and lowest sum(q), and by 2^-21 of the
+    exponential's. Weights are off by that of their own and the mean one, relatively. A value enters as (code - 8) step and
+    low + 8 step, times its weight, rounded to u' = 2^-21 (fp32 queries), or to 2^-11 where 16-bit queries take p * step
+    in one fp16; products below 2^-16 of a row's largest lose up to 2^-27 of that."""
+    k, v = (x[:, 0] for x in c.get(0, n))
+    G = k.shape[1] // 64
+    codes = ref.unpack(c.k[0, 0, :n]).double().unflatten(-1, (G, 64))
+    ks, kl = (c.kp[0, 0, :n, :, i].double() for i in (0, 1))
+    step, low = (c.vp[0, 0, :n, :, i].double() for i in (0, 1))
+    size = 8 * step + (low + 8 * step).abs()  # [n, G]
+    qd = q.double()
+    up = 2.0 ** (bits - 1 - torch.floor(torch.log2(qd.abs().amax(-1, keepdim=True))))
+    left = (qd * up - torch.round(qd * up)).abs() / up
+    x = qd @ k.T * scale
+    w = torch.softmax(x, -1)
+    qg = qd.unflatten(-1, (G, 64))
+    parts = sum(ks[:, g] * (qg[:, g] @ codes[:, g].T).abs() + (kl[:, g] * qg[:, g].sum(-1, keepdim=True)).abs() for g in range(G))
+    e = scale * (left @ k.abs().T + 6 * 2.0 ** -24 * parts) + 2.0 ** -21
+    e = e + (w * e).sum(-1, keepdim=True)
+    u1 = {"f32": 2.0 ** -21, "f16": 2.0 ** -11, "bf16": 2.0 ** -11}[typ]
+    lost = 8 * n * 2.0 ** -27 * (w[:, :, None] * step).amax(1)
+    tol = (w * (e + u1)) @ size + lost  # [H, G]
+    want = w @ v
+    u = {"f32": 2.0 ** -23, "f16": 2.0 ** -10, "bf16": 2.0 ** -7}[typ]
+    tiny = 2.0 ** -25 if typ == "f16" else 1e-37
+    return tol.repeat_interleave(64, -1) + u / 2 * want.abs() + tiny, want
+
+
+def kv4_digits(on, c, q, n, typ, scale):
+    from test_gpu_longctx import attn4
+
+    rc, out = attn4(on, c, q[None, None], [n], typ, scale=scale)
+    assert rc == 0 and on.L.ork_b200_sync(on.ctx) == 0
+    tol, want = kv4_error_bound(c, q, n, typ, scale)
+    err = (out[0, 0].double() - want).abs()
+    assert (err <= tol).all(), (float((err / tol).max()), float(err.max()))
+    return tol, want
+
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("small", [0, 1])
+@pytest.mark.parametrize("ratio", [1.0, 1e4, 1e6])
+def test_kv4_attn_a_group_of_small_values_keeps_its_digits(on, typ, small, ratio):
+    # queries in sixteenths are exact as integers, which leaves the values' digits
+    from test_gpu_longctx import Cache
+
+    n, dk = 3000, 128
+    c = Cache(1, 1, dk, 3008)
+    v = rnd((n, 1, dk), 490, 1e4)
+    v[:, :, 64 * small:64 * small + 64] /= ratio
+    c.put(0, rnd((n, 1, dk), 491), v)
+    q = (torch.round(rnd((8, dk), 492, 16.0)) / 16).to(DT[typ])
+    kv4_digits(on, c, q, n, typ, dk ** -0.5)
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("groups", [(0, 1), (1,)])
+@pytest.mark.parametrize("at", [0, 700, 2999])
+def test_kv4_attn_a_large_value_without_weight_costs_no_digits(on, typ, groups, at):
+    # one token's values a million times the others', and next to no weight on it
+    from test_gpu_longctx import Cache
+
+    n, dk = 3000, 128
+    c = Cache(1, 1, dk, 3008)
+    k, v = rnd((n, 1, dk), 493), rnd((n, 1, dk), 494, 0.01)
+    q = (torch.round(rnd((dk,), 495, 16.0)) / 16).to(DT[typ]).expand(8, dk).contiguous()
+    k[at, 0] = -8 * q[0].float()
+    for g in groups:
+        v[at, :, 64 * g:64 * g + 64] *= 1e6
+    c.put(0, k, v)
+    kv4_digits(on, c, q, n, typ, dk ** -0.5)
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("sink", [0.0, 0.01, 1.0])
+@pytest.mark.parametrize("at", [0, 20000])
+def test_kv4_attn_a_long_tail_far_below_one_token(on, typ, sink, at):
+    # a token 17 nats above 32767 others, whose output is theirs where its values are 0
+    from test_gpu_longctx import Cache
+
+    n, dk = 32768, 64
+    c = Cache(1, 1, dk, n)
+    k, v = rnd((n, 1, dk), 496, 0.2), rnd((n, 1, dk), 497, 30.0)
+    q = (torch.round(rnd((dk,), 498, 16.0)) / 16).to(DT[typ]).expand(5, dk).contiguous()
+    k[at, 0] = q[0].float() / float(q[0].float().norm()) ** 2 * 17.0 * 8.0
+    v[at] *= sink
+    c.put(0, k, v)
+    kv4_digits(on, c, q, n, typ, 0.125)
