@@ -195,8 +195,10 @@ int ork_b200_kv4_load_async(ork_npu *ctx, const ork_b200_kv4 *c, void *k, void *
  * prompt's rows). Sequence s holds len[s] tokens (device int [nseq], at most max_len, the new ones among them; 0
  * leaves its rows zero); token t of T is at position len[s] - T + t and sees keys as in ork_b200_attn. q row (s, t)
  * of head h lies at q + (s*T + t) * q_ts + h * q_hs; out is [nseq][T][H][dk]. q and out have `type`, any of the
- * three, and are aligned to it; arithmetic is fp32-like throughout (operands of the matrix instructions are split
- * in two halves). After an eviction positions count the kept tokens.
+ * three, and are aligned to it; out overlaps no input. After an eviction positions count the kept tokens. Arithmetic:
+ * a query row enters as integers of 29 bits (ORK_B200_F32) or 21 below its largest magnitude, the logits, the softmax
+ * and all sums are fp32, and a token's weight times the step of its values enters the second product in two fp16 (22
+ * bits; ORK_B200_F32) or in one (11 bits), the step of each 64 dims scaled by itself.
  * wsum (NULL: none) [nseq][Hkv][cap] fp32: every visible key's softmax weights, summed over the T tokens and the
  * H / Hkv heads of its kv head, are added to its entry. */
 typedef struct ork_b200_kv4_attn {

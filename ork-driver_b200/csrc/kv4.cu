@@ -261,7 +261,9 @@ __global__ void __launch_bounds__(kRowThreads, STORE ? 4 : 1) kv4_rows_kernel(Ro
 // rows than that per kv head, and the other way round half of each product would be padding.
 // First product, mma.m16n8k32 of 8-bit integers: an AND takes four codes out of a word. q is scaled per row to
 // integers below 2^21 and split into three signed bytes; the three products run one after another, the sums shifted
-// left by eight between them, and stay below 2^31: the logits carry q's 21 bits and no other error. (A code in the
+// left by eight between them, and stay below 2^31: the logits carry q's 21 bits and no other error. fp32 queries have a
+// fourth byte, summed by itself: 29 bits, so that a dim keeps fp32's digits next to one 32 times larger, and 22 bits
+// next to one 128 times larger (a dim of 200 among dims of 1.6: outputs off by 3e-6, 4e-5 with three bytes). (A code in the
 // low bits of an fp16 is an exact subnormal too, and one instruction fewer; but the tensor cores align what they add
 // by the nominal exponents, and the leading zeros cost 6 to 10 of their 24 bits: logits were off by 2^-15.)
 // Second product, mma.m16n8k16 of fp16: the output has no more than 11 bits either. A shift and two ANDs put two nibbles
@@ -437,13 +439,15 @@ constexpr int kStages = DK == 128 ? 2 : 4;
 template <class E, int DK, int NT>
 constexpr int kCtas = DK == 128 && (NT == 2 || sizeof(E) == 4) ? 2 : 3;
 // q of a CTA: its bytes in the order the first product takes them, and the scales and sums of its rows
-template <int DK, int NT>
+template <class E>
+constexpr int kDigits = sizeof(E) == 4 ? 4 : 3;
+template <class E, int DK, int NT>
 struct Query {
-  uint4 d[NT][3][DK / kGroup][32];
+  uint4 d[NT][kDigits<E>][DK / kGroup][32];
   float f[NT * kRows], sum[DK / kGroup][NT * kRows];
 };
-template <int DK, int NT>
-constexpr int kAttnSmem = kWarps * (kStages<DK> * ((int)sizeof(Stage<DK>) + 8) + (int)sizeof(Wide<DK>)) + (int)sizeof(Query<DK, NT>);
+template <class E, int DK, int NT>
+constexpr int kAttnSmem = kWarps * (kStages<DK> * ((int)sizeof(Stage<DK>) + 8) + (int)sizeof(Wide<DK>)) + (int)sizeof(Query<E, DK, NT>);
 
 template <int N>
 __device__ __forceinline__ void load_pars(const float *p, float (&x)[N]) {
@@ -493,6 +497,7 @@ template <class E, int DK, int NT, bool WS>
 __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel(const Attn4 a, const E *__restrict__ q, E *__restrict__ out) {
   constexpr int NG = DK / kGroup, NST = kStages<DK>, TR = NT * kRows;
   constexpr bool SPLIT = sizeof(E) == 4;
+  constexpr int ND = kDigits<E>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // known to be the same for the whole warp
@@ -500,7 +505,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   const int s = blockIdx.y, G = a.H / a.Hkv, rows = a.T * G;
   Stage<DK> *ring = reinterpret_cast<Stage<DK> *>(smem) + warp * NST;
   Wide<DK> *wide = reinterpret_cast<Wide<DK> *>(smem + kWarps * NST * sizeof(Stage<DK>)) + warp;
-  Query<DK, NT> *qm = reinterpret_cast<Query<DK, NT> *>(smem + kWarps * (NST * sizeof(Stage<DK>) + sizeof(Wide<DK>)));
+  Query<E, DK, NT> *qm = reinterpret_cast<Query<E, DK, NT> *>(smem + kWarps * (NST * sizeof(Stage<DK>) + sizeof(Wide<DK>)));
   const uint32_t bars = sm100::smem_addr(qm + 1) + warp * NST * 8;
   // q of row r of tile y, by warp y: on its way while the sequence's length is read
   float qx[NG][16];
@@ -542,7 +547,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
       next += cnt;
     }
 
-  // as integers: byte 2 - d of those of the lane's words, even dims then odd ones
+  // as integers: byte ND - 1 - d of those of the lane's words, even dims then odd ones
   if (warp < NT) {
     const int y = warp;
     float mx = 0.0f;
@@ -557,25 +562,26 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
     mx = quad_max(mx);
     const unsigned quad = 15u << (lane & 28);
     fin = (__ballot_sync(0xffffffffu, fin) & quad) == quad;
-    const int e = fin ? min(100, 147 - (int)(__float_as_uint(mx) >> 23)) : 0;  // -107 at least
+    const int e = fin ? min(100, 123 + 8 * ND - (int)(__float_as_uint(mx) >> 23)) : 0;  // -107 at least
     const float up = pow2(e), f = fin ? a.scale * 1.4426950408889634f * pow2(-e) : __int_as_float(0x7fc00000);
     if (c == 0) qm->f[y * kRows + r] = f;
 #pragma unroll
     for (int g = 0; g < NG; g++) {
-      int w[16], sum = 0;
+      int w[16];
+      std::conditional_t<SPLIT, long long, int> sum = 0;
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         w[i] = fin ? __float2int_rn(qx[g][i] * up) : 0;
         sum += w[i];
-        w[i] += 0x808080;  // bytes of 128 + digit
+        w[i] = (int)((uint32_t)w[i] + (ND == 4 ? 0x80808080u : 0x808080u));  // bytes of 128 + digit
       }
       const float total = quad_sum((float)sum) * f;
       if (c == 0) qm->sum[g][y * kRows + r] = total;
 #pragma unroll
-      for (int d = 0; d < 3; d++) {
+      for (int d = 0; d < ND; d++) {
         auto digit = [&](int i) {
           const int w4[4] = {w[i], w[i + 2], w[i + 4], w[i + 6]};
-          return bytes_of(w4, 2 - d) ^ 0x80808080u;
+          return bytes_of(w4, ND - 1 - d) ^ 0x80808080u;
         };
         qm->d[y][d][g][lane] = make_uint4(digit(0), digit(1), digit(8), digit(9));
       }
@@ -704,7 +710,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
     const int mt = (r >> 1) + 4 * (r & 1);
 #pragma unroll
     for (int w = 0; w < kStageUnits; w++) {  // units past cnt hold old codes, and steps of zero
-      int acc[NT][NG][4];
+      int acc[NT][NG][4], low[SPLIT ? NT : 1][NG][4];  // of the first three digits; of the fourth
 #pragma unroll
       for (int g = 0; g < NG; g++) {
         const uint8_t *kr = st->k + (kUnit * w + mt) * (DK / 2) + g * 32 + c * 8;
@@ -715,11 +721,16 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
 #pragma unroll
         for (int y = 0; y < NT; y++)
 #pragma unroll
-          for (int d = 0; d < 3; d++) {
+          for (int d = 0; d < ND; d++) {
             uint32_t qb[4];  // kept in shared memory, the registers are full
             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(qb[0]), "=r"(qb[1]), "=r"(qb[2]), "=r"(qb[3])
-                         : "r"(qaddr + (uint32_t)(((y * 3 + d) * NG + g) * 512)));
+                         : "r"(qaddr + (uint32_t)(((y * ND + d) * NG + g) * 512)));
+            if (d == 3) {
+              mma_i80(low[SPLIT ? y : 0][g], af[0], qb[0], qb[1]);
+              mma_i8(low[SPLIT ? y : 0][g], af[1], qb[2], qb[3]);
+              continue;
+            }
             if (d == 0) mma_i80(acc[y][g], af[0], qb[0], qb[1]);
             else {
 #pragma unroll
@@ -737,9 +748,13 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
         for (int y = 0; y < NT; y++)
 #pragma unroll
           for (int i = 0; i < 2; i++) {
-            float d = (float)acc[y][0][2 * h + i] * par[0], b = par[NG] * qs[y][0][i];
+            auto dot = [&](int g) {  // q . codes
+              const float top = (float)acc[y][g][2 * h + i];
+              return SPLIT ? fmaf(top, 256.0f, (float)low[SPLIT ? y : 0][g][2 * h + i]) : top;
+            };
+            float d = dot(0) * par[0], b = par[NG] * qs[y][0][i];
             if constexpr (NG == 2) {
-              d = fmaf((float)acc[y][1][2 * h + i], par[1], d);
+              d = fmaf(dot(1), par[1], d);
               b = fmaf(par[NG + 1], qs[y][1][i], b);
             }
             x[y][w][2 * h + i] = fmaf(d, fs[y][i], b);
@@ -1149,7 +1164,7 @@ int choose_splits(const Attn4 &a, int ctas) {
 template <class E, int DK, bool WS>
 cudaError_t launch_attn_ws(const Attn4 &a, const E *q, E *out, cudaStream_t st, uint64_t *launches) {
   auto kern = a.prow / a.tiles == kRows ? kv4_attn_kernel<E, DK, 1, WS> : kv4_attn_kernel<E, DK, 2, WS>;
-  const int smem = a.prow / a.tiles == kRows ? kAttnSmem<DK, 1> : kAttnSmem<DK, 2>;
+  const int smem = a.prow / a.tiles == kRows ? kAttnSmem<E, DK, 1> : kAttnSmem<E, DK, 2>;
   cudaError_t e = smem_attr((const void *)kern, smem);
   if (e != cudaSuccess) return e;
   kern<<<dim3(a.splits * a.tiles * a.Hkv, a.nseq), 32 * kWarps, smem, st>>>(a, q, out);

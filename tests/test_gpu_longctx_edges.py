@@ -300,12 +300,12 @@ def kv4_error_bound(c, q, n, typ, scale, bits=21):
     return tol.repeat_interleave(64, -1) + u / 2 * want.abs() + tiny, want
 
 
-def kv4_digits(on, c, q, n, typ, scale):
+def kv4_digits(on, c, q, n, typ, scale, bits=21):
     from test_gpu_longctx import attn4
 
     rc, out = attn4(on, c, q[None, None], [n], typ, scale=scale)
     assert rc == 0 and on.L.ork_b200_sync(on.ctx) == 0
-    tol, want = kv4_error_bound(c, q, n, typ, scale)
+    tol, want = kv4_error_bound(c, q, n, typ, scale, bits)
     err = (out[0, 0].double() - want).abs()
     assert (err <= tol).all(), (float((err / tol).max()), float(err.max()))
     return tol, want
@@ -363,3 +363,16 @@ def test_kv4_attn_a_long_tail_far_below_one_token(on, typ, sink, at):
     v[at] *= sink
     c.put(0, k, v)
     kv4_digits(on, c, q, n, typ, 0.125)
+
+
+@pytest.mark.parametrize("dk,H", [(64, 3), (128, 8), (64, 16), (128, 11)])
+@pytest.mark.parametrize("n", [8, 50])
+def test_kv4_attn_fp32_queries_keep_digits_next_to_large_ones(on, dk, H, n):
+    # two dims far above the others that cancel in every logit: integers of 29 bits below them leave the others theirs
+    from test_gpu_longctx import Cache
+
+    c = Cache(1, 1, dk, 64)
+    k, q = rnd((n, 1, dk), 500), rnd((H, dk), 501, 1.6)
+    q[:, 5], q[:, 9], k[..., 5], k[..., 9] = 1000.0, -1000.0, 0.25, 0.25
+    c.put(0, k, rnd((n, 1, dk), 502))
+    kv4_digits(on, c, q, n, "f32", dk ** -0.5, 29)
