@@ -200,7 +200,9 @@ int ork_b200_kv4_load_async(ork_npu *ctx, const ork_b200_kv4 *c, void *k, void *
  * and all sums are fp32, and a token's weight times the step of its values enters the second product in two fp16 (22
  * bits; ORK_B200_F32) or in one (11 bits), the step of each 64 dims scaled by itself.
  * wsum (NULL: none) [nseq][Hkv][cap] fp32: every visible key's softmax weights, summed over the T tokens and the
- * H / Hkv heads of its kv head, are added to its entry. */
+ * H / Hkv heads of its kv head, are added to its entry. The workspace then holds the logits of all rows, 4 GiB at a time
+ * (a call of more goes through its tokens in passes). Every 16 rows (tokens times H / Hkv) of a kv head read the cache
+ * once: many tokens after a prefix are the prompt attention's work. */
 typedef struct ork_b200_kv4_attn {
   const void *q;
   void *out;

@@ -321,6 +321,7 @@ struct Attn4 {
   const uint8_t *kc, *vc;
   const __half *kp, *vp;
   int nseq, Hkv, cap, H, T, window, sinks, max_len;
+  int row_T, late;  // rows of q and out from one sequence to the next; tokens held that come after the T ones
   long long q_ts, q_hs;
   const int *len;
   float scale;
@@ -353,10 +354,10 @@ __device__ __forceinline__ int token_of(const Units &u, int unit) {
   return (unit < u.su ? unit : unit - u.su + u.lo) * kUnit;
 }
 
-// the number of tokens of sequence s; 0 (reported) where it cannot be
+// the number of tokens of sequence s up to the last of T; 0 (reported) where it cannot be
 __device__ __forceinline__ int seq_len(const Attn4 &a, int s) {
   const int n = a.len[s];
-  if (n >= 0 && n <= a.max_len) return n;
+  if (n >= 0 && n <= a.max_len) return max(n - a.late, 0);
   if (threadIdx.x == 0) kv4_error();
   return 0;
 }
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   float qx[NG][16];
   if (warp < NT) {
     const int row = tile * TR + warp * kRows + r;
-    const E *qr = q + ((long long)s * a.T + row / G) * a.q_ts + (long long)(kvh * G + row % G) * a.q_hs + 16 * c;
+    const E *qr = q + ((long long)s * a.row_T + row / G) * a.q_ts + (long long)(kvh * G + row % G) * a.q_hs + 16 * c;
 #pragma unroll
     for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -963,7 +964,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   __syncthreads();
   constexpr int PER = 8;  // consecutive dims of one row
   auto write_row = [&](int row, int d0, float m, float sum, const float (&v)[PER]) {
-    E *dst = out + (((long long)s * a.T + row / G) * a.H + kvh * G + row % G) * DK + d0;
+    E *dst = out + (((long long)s * a.row_T + row / G) * a.H + kvh * G + row % G) * DK + d0;
 #pragma unroll
     for (int i = 0; i < PER; i++) dst[i] = from_f32<E>(sum == 0.0f ? 0.0f : v[i] / sum);
     if (WS && d0 == 0) a.stat[((size_t)s * a.Hkv + kvh) * a.prow + row] = m == -INFINITY ? sum : m + log2f(sum);
@@ -1092,7 +1093,7 @@ __device__ __forceinline__ void join_row(const Attn4 &a, E *__restrict__ out) {
     sum = fmaf(k, sml[w].y, sum);
     if (k != 0.0f) x = fmaf(k, so[w][threadIdx.x], x);
   }
-  out[(((long long)s * a.T + row / G) * a.H + kvh * G + row % G) * DK + threadIdx.x] = from_f32<E>(sum == 0.0f ? 0.0f : x / sum);
+  out[(((long long)s * a.row_T + row / G) * a.H + kvh * G + row % G) * DK + threadIdx.x] = from_f32<E>(sum == 0.0f ? 0.0f : x / sum);
 }
 
 __device__ __forceinline__ void sum_weights(const Attn4 &a, int block) {
@@ -1267,6 +1268,42 @@ static int kv4_rows(ork_npu *c, const ork_b200_kv4 *kv, const void *k, const voi
   return 0;
 }
 
+// What a launch for the tokens t0 .. t0 + T - 1 of the call's T takes, and where in the workspace (from 0 on).
+struct Plan4 {
+  Attn4 k;
+  size_t ml, po, stat, need;  // bytes of partial maxima, outputs, statistics; of all
+  size_t counts;
+};
+static Plan4 kv4_plan(const ork_b200_kv4 *kv, const ork_b200_kv4_attn *a, int t0, int T) {
+  Plan4 p = {};
+  Attn4 &k = p.k;
+  k.kc = kv->k, k.vc = kv->v, k.kp = (const __half *)kv->kp, k.vp = (const __half *)kv->vp;
+  k.nseq = kv->nseq, k.Hkv = kv->Hkv, k.cap = kv->cap, k.H = a->H, k.T = T, k.row_T = a->T, k.late = a->T - t0 - T;
+  k.window = a->window < a->max_len ? a->window : 0;  // a window over everything is none
+  k.sinks = std::min(a->sinks, a->max_len);
+  k.max_len = a->max_len, k.q_ts = a->q_ts, k.q_hs = a->q_hs, k.len = a->len, k.scale = a->scale, k.wsum = a->wsum;
+  const int rows = T * (a->H / kv->Hkv), tr = rows > kRows ? 2 * kRows : kRows;
+  k.tiles = (rows + tr - 1) / tr;
+  k.prow = k.tiles * tr;
+  // sinks and window, whole units of each
+  long long vis = (std::max(a->max_len - k.late, 1) + kUnit - 1) / kUnit * kUnit;
+  if (k.window) vis = std::min<long long>(vis, (long long)k.window + k.T + k.sinks + 3 * kUnit);
+  k.vis = (int)(vis / kUnit * kUnit);
+  k.splits = choose_splits(k, kv->dk == 128 && (tr > kRows || a->type == ORK_B200_F32) ? 2 : 3);
+  k.qvec = ((uintptr_t)a->q | (size_t)a->q_ts * elem_bytes(a->type) | (size_t)a->q_hs * elem_bytes(a->type)) % 16 == 0;
+  k.join = k.splits > 1 && k.splits <= kJoinSplits;
+  auto whole = [](size_t b) { return (b + 255) / 256 * 256; };
+  const size_t prows = (size_t)k.nseq * k.Hkv * k.prow, parts = k.splits > 1 ? prows * k.splits : 0;
+  p.ml = whole(parts * sizeof(float2)), p.po = whole(parts * kv->dk * 4), p.stat = a->wsum ? whole(prows * 4) : 0;
+  p.need = p.ml + p.po + p.stat + (a->wsum ? prows * k.vis * 4 : 0);
+  if (k.join || (a->wsum && k.splits > 1)) p.counts = (size_t)k.nseq * k.Hkv * k.tiles;
+  return p;
+}
+
+// Logits that a call with weights to add up keeps at a time, in bytes: a call of more goes through its tokens in several
+// passes (2500 tokens of 16 heads after 60000: 9.6 GB otherwise). Decode steps and drafts need one.
+constexpr long long kLogits = 4ll << 30;
+
 extern "C" {
 
 int ork_b200_kv4_store_async(ork_npu *c, const ork_b200_kv4 *kv, const void *k, const void *v, int type, int rows,
@@ -1298,41 +1335,36 @@ int ork_b200_kv4_attn_async(ork_npu *c, const ork_b200_kv4 *kv, const ork_b200_k
     if (e != cudaSuccess) log_err(name, e);
     return e == cudaSuccess ? 0 : -1;
   }
-  Attn4 k = {};
-  k.kc = kv->k, k.vc = kv->v, k.kp = (const __half *)kv->kp, k.vp = (const __half *)kv->vp;
-  k.nseq = kv->nseq, k.Hkv = kv->Hkv, k.cap = kv->cap, k.H = a->H, k.T = a->T;
-  k.window = a->window < a->max_len ? a->window : 0;  // a window over everything is none
-  k.sinks = std::min(a->sinks, a->max_len);
-  k.max_len = a->max_len, k.q_ts = a->q_ts, k.q_hs = a->q_hs, k.len = a->len, k.scale = a->scale, k.wsum = a->wsum;
-  const int rows = a->T * (a->H / kv->Hkv), tr = rows > kRows ? 2 * kRows : kRows;
-  k.tiles = (rows + tr - 1) / tr;
-  k.prow = k.tiles * tr;
-  // sinks and window, whole units of each
-  long long vis = (a->max_len + kUnit - 1) / kUnit * kUnit;
-  if (k.window) vis = std::min<long long>(vis, (long long)k.window + k.T + k.sinks + 3 * kUnit);
-  k.vis = (int)(vis / kUnit * kUnit);
-  k.splits = choose_splits(k, kv->dk == 128 && (tr > kRows || a->type == ORK_B200_F32) ? 2 : 3);
-  k.qvec = ((uintptr_t)a->q | (size_t)a->q_ts * elem_bytes(a->type) | (size_t)a->q_hs * elem_bytes(a->type)) % 16 == 0;
-  k.join = k.splits > 1 && k.splits <= kJoinSplits;
-  auto whole = [](size_t b) { return (b + 255) / 256 * 256; };
-  const size_t prows = (size_t)k.nseq * k.Hkv * k.prow, parts = k.splits > 1 ? prows * k.splits : 0;
-  const size_t mlb = whole(parts * sizeof(float2)), pob = whole(parts * kv->dk * 4), stb = a->wsum ? whole(prows * 4) : 0;
-  const size_t need = mlb + pob + stb + (a->wsum ? prows * k.vis * 4 : 0);
-  if (need && !work_block(c, name, &c->work, need)) return -1;
-  if (k.join || (a->wsum && k.splits > 1)) {
-    unsigned int *z = zeroed_counts(c, name, (size_t)k.nseq * k.Hkv * k.tiles);
-    if (!z) return -1;
-    k.done = z + kAttnCounts;
+  int step = a->T;  // tokens a pass
+  if (a->wsum) {
+    const long long span = a->window ? std::min<long long>(a->max_len, (long long)a->window + a->T + a->sinks + 3 * kUnit) : a->max_len;
+    int unit = 1;  // tokens of whole column tiles
+    while (unit < 2 * kRows && (a->H / kv->Hkv) * unit % (2 * kRows)) unit *= 2;
+    step = (int)std::min<long long>(step, std::max(kLogits / ((long long)kv->nseq * a->H * span * 4) / unit, 1ll) * unit);
   }
-  uint8_t *ws = (uint8_t *)c->work.p;
-  k.pml = (float2 *)ws, k.po = (float *)(ws + mlb), k.stat = (float *)(ws + mlb + pob), k.x = (float *)(ws + mlb + pob + stb);
-  const cudaError_t e = with_elem(a->type, [&](auto *t) {
-    using E = std::remove_pointer_t<decltype(t)>;
-    return launch_attn<E>(k, kv->dk, (const E *)a->q, (E *)a->out, c->stream, &c->launches);
-  });
-  if (e != cudaSuccess) {
-    log_err(name, e);
-    return -1;
+  Plan4 p = kv4_plan(kv, a, 0, step);
+  size_t need = p.need, counts = p.counts;
+  for (int t = step; t < a->T; t += step) {  // whatever is refused is refused before the first pass
+    const Plan4 q = kv4_plan(kv, a, t, std::min(step, a->T - t));
+    need = std::max(need, q.need), counts = std::max(counts, q.counts);
+  }
+  if (need && !work_block(c, name, &c->work, need)) return -1;
+  unsigned int *done = nullptr;
+  if (counts && !(done = zeroed_counts(c, name, counts))) return -1;
+  for (int t = 0; t < a->T; t += step) {
+    if (t) p = kv4_plan(kv, a, t, std::min(step, a->T - t));
+    uint8_t *ws = (uint8_t *)c->work.p;
+    p.k.pml = (float2 *)ws, p.k.po = (float *)(ws + p.ml), p.k.stat = (float *)(ws + p.ml + p.po);
+    p.k.x = (float *)(ws + p.ml + p.po + p.stat);
+    p.k.done = done + kAttnCounts;
+    const cudaError_t e = with_elem(a->type, [&](auto *x) {
+      using E = std::remove_pointer_t<decltype(x)>;
+      return launch_attn<E>(p.k, kv->dk, (const E *)a->q + t * a->q_ts, (E *)a->out + (long long)t * a->H * kv->dk, c->stream, &c->launches);
+    });
+    if (e != cudaSuccess) {
+      log_err(name, e);
+      return -1;
+    }
   }
   return 0;
 }

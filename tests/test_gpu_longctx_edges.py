@@ -376,3 +376,30 @@ def test_kv4_attn_fp32_queries_keep_digits_next_to_large_ones(on, dk, H, n):
     q[:, 5], q[:, 9], k[..., 5], k[..., 9] = 1000.0, -1000.0, 0.25, 0.25
     c.put(0, k, rnd((n, 1, dk), 502))
     kv4_digits(on, c, q, n, "f32", dk ** -0.5, 29)
+
+
+@pytest.mark.parametrize("T,H,Hkv,lens,window,sinks,cap", [(70, 8, 1, [500, 71, 30, 0], 0, 0, 512), (33, 12, 4, [1000, 5], 200, 7, 1024),
+                                                          (300, 3, 3, [333, 299], 0, 0, 384)])
+def test_kv4_attn_many_tokens(on, T, H, Hkv, lens, window, sinks, cap):
+    # hundreds of rows a kv head, sequences shorter than the tokens among them
+    from test_gpu_longctx import Cache, attn4_check
+
+    c = Cache(len(lens), Hkv, 64, cap)
+    for s, n in enumerate(lens):
+        c.put(s, rnd((n, Hkv, 64), 510 + s), rnd((n, Hkv, 64), 515 + s))
+    attn4_check(on, c, rnd((len(lens), T, H, 64), 520, 1.5), lens, "f32", window, sinks)
+
+
+def test_kv4_attn_weights_of_many_tokens_in_bounded_memory(on):
+    # 9.6 GB of logits: in passes, with a workspace of 4 GiB and half as much again at most; one sequence is shorter than
+    # the tokens of the first pass
+    from test_gpu_longctx import Cache, attn4_check
+
+    T, lens, cap = 2500, [30000, 1200], 30016
+    with B.Context() as own:
+        own.L.ork_b200_set_stream(own.ctx, 1)
+        c = Cache(2, 2, 64, cap)
+        for s, n in enumerate(lens):
+            c.put(s, rnd((n, 2, 64), 530 + s), rnd((n, 2, 64), 532 + s))
+        attn4_check(own, c, rnd((2, T, 16, 64), 534, 1.5, torch.float16), lens, "f16")
+        assert own.L.ork_b200_staging_bytes(own.ctx) < 6.5e9
