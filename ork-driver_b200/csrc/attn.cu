@@ -26,7 +26,8 @@
 // 1024: 390 us. Measured against: a step of 64 keys with two places for S, 1.58 ms; P handed over by halves, 1.02 ms;
 // two threads a row, 0.93 to 1.02 ms.
 //
-// Every wait is bounded; one that expires records an error and the roles fall through to the common exit.
+// Every wait is bounded; one that expires records an error and the roles fall through to the common exit, which waits,
+// bounded too, for the copies and products still on their way.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
@@ -118,7 +119,7 @@ struct Smem {
   static constexpr int kSlots = DK == 128 ? 4 : 8;
   static constexpr int kTileBytes = kTile * DK * 2, kChunk = kTile * 128;  // a 64-column block of a tile
   static constexpr int kStage = (2 + kSlots) * kTileBytes, kBar = kStage + 8 * 4096;
-  static constexpr int kBars = 2 + 2 * kSlots + 6 + 4, kItem = kBar + kBars * 8;
+  static constexpr int kBars = 2 + 2 * kSlots + 6 + 4 + 2, kItem = kBar + kBars * 8;
   static constexpr int kList = kItem + 2 * 80 + 16, kBytes = 1024 + kList + 8 * 16;
 };
 static_assert(Smem<128>::kBytes <= 232448 && Smem<64>::kBytes <= 232448, "shared memory");
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sq = sm100::smem_addr(smem), sring = sq + 2 * M::kTileBytes, bars = sq + M::kBar;
   const uint32_t qfull = bars, qempty = bars + 8, full = bars + 16, empty = full + 8 * SLOTS, sfull = empty + 8 * SLOTS,
-                 pfull = sfull + 16, ofull = pfull + 16, ifull = ofull + 16, iempty = ifull + 16;
+                 pfull = sfull + 16, ofull = pfull + 16, ifull = ofull + 16, iempty = ifull + 16, done = iempty + 16;
   Item *place = (Item *)(smem + M::kItem);  // [2]
   uint32_t *slot = (uint32_t *)(smem + M::kItem + 2 * 80);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -292,6 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm100::bar_init(sfull + 8 * t, 1), sm100::bar_init(pfull + 8 * t, 4);
       sm100::bar_init(ofull + 8 * t, 1), sm100::bar_init(ifull + 8 * t, 1), sm100::bar_init(iempty + 8 * t, 9);
     }
+    sm100::bar_init(done, 1);
     sm100::bar_init_fence();
   }
   // the items of which the warp has rows to compute again: how many, the latest one's number and first such row. That row
@@ -341,6 +343,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the last CTA to be done with the count leaves it zero for the next launch
       __threadfence();
       if (atomicInc(count + 1, gridDim.x - 1) == gridDim.x - 1) *count = 0;
+      // no copy is on its way when the CTA ends, whoever gave up
+      if (nq) sm100::bar_wait(qfull, (nq - 1) & 1);
+      for (int i = max(0, g - SLOTS); i < g; i++) sm100::bar_wait(full + 8 * (i % SLOTS), (i / SLOTS) & 1);
     } else if (warp == 8) {  // ---- products, issued by one elected lane from operands the whole warp agrees on
       constexpr uint32_t ids = inst_desc<E>(kTile, false), ido = inst_desc<E>(DK, true);
       constexpr uint32_t kSlot = M::kTileBytes >> 4;
@@ -440,6 +445,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
       if (!ok && lane == 0) attn_failed();
+      if (sm100::elect_one()) sm100::tc_commit(done);  // nor a product
+      __syncwarp();
+      sm100::bar_wait(done, 0);
     }
   } else {  // ---- softmax of tile t, a thread per row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");

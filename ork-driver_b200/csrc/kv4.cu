@@ -927,7 +927,14 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
     }
     if (++slot == NST) slot = 0, parity ^= 1;
   }
-  if (!ok && lane == 0) kv4_error();
+  if (!ok) {
+    if (lane == 0) kv4_error();
+#pragma unroll 1
+    for (int i = 0; i < NST; i++) {  // copies still on their way land before the rings are used again, if they ever do
+      sm100::bar_wait(bars + 8 * slot, parity);
+      if (++slot == NST) slot = 0, parity ^= 1;
+    }
+  }
 
   // ---- the warps' results, then the CTA's
   sm100::dependents_launch();
