@@ -34,6 +34,22 @@ def test_evict_updates_lengths_in_place(on, nseq, Hkv, n, keep):
             assert kept[s, h].tolist() == at + [-1] * (keep - len(at)), (s, h)
 
 
+def test_evict_of_more_keys_than_a_block_holds(on):
+    # so many heads that each gets one block, and so many tokens that it reads the scores anew in every pass
+    nseq, Hkv, n, keep = 19, 8, 25000, 500
+    score = torch.exp(rnd((nseq, Hkv, n), 404, 3))
+    score[:, 0] = torch.floor(score[:, 0])  # many ties
+    ln, kept = ints([n - 7 * s for s in range(nseq)]), torch.zeros((nseq, Hkv, keep), dtype=torch.int32, device="cuda")
+    e = B.Evict(score=score.data_ptr(), len=ln.data_ptr(), nseq=nseq, Hkv=Hkv, cap=n, dcap=keep, max_len=n, keep=keep, sinks=4,
+                recent=64, nplanes=0, kept=kept.data_ptr(), len_out=ln.data_ptr())
+    assert on.L.ork_b200_evict_async(on.ctx, C.byref(e)) == 0 and on.L.ork_b200_sync(on.ctx) == 0
+    assert ln.tolist() == [keep] * nseq
+    sc, kept = score.cpu(), kept.cpu()
+    for s in range(0, nseq, 3):
+        for h in (0, 1 + s % 7):
+            assert kept[s, h].tolist() == evict_want(sc[s, h], n - 7 * s, keep, 4, 64), (s, h)
+
+
 # ---- CUDA graphs and the workspace --------------------------------------------------------------------------------
 
 def cache(nseq, Hkv, dk, cap, seed):
