@@ -139,8 +139,8 @@ int ork_b200_argmax_scaled_async(ork_npu *ctx, const int32_t *C, const float *bs
  * ork_b200_sync. Calls on one context share a workspace and counters, which the first call of a larger size allocates:
  * they run one after another, and one call of each size is made before a CUDA graph captures it (a capture that would
  * need more is refused). What a captured call was given stays allocated until the context is freed, so that its graph
- * can be replayed whatever is called in between. `type` is one of the three below; strides are in elements. Head size dk is 64 or 128; query head
- * h reads kv head h / (H / Hkv), so H is a multiple of Hkv. */
+ * can be replayed whatever is called in between. `type` is one of the three below; strides are in elements. Head size
+ * dk is 64 or 128; query head h reads kv head h / (H / Hkv), so H is a multiple of Hkv. */
 #define ORK_B200_F32 0
 #define ORK_B200_F16 1
 #define ORK_B200_BF16 2
@@ -153,8 +153,7 @@ int ork_b200_argmax_scaled_async(ork_npu *ctx, const int32_t *C, const float *bs
  * head h lies at q + r * q_ts + h * q_hs, its dk values contiguous, likewise k, v and out.
  * type ORK_B200_F16 or ORK_B200_BF16 (inputs and output); scale is positive; the scores and the output are summed in
  * fp32 and the softmax weights enter the second product rounded to `type` (fp16: to 2^-32 of the row's largest at best).
- * Bases are 16-byte aligned, strides multiples of 8.
- * out overlaps no input. q_start, k_start: device int [nseq + 1]; q_rows / k_rows: rows that q and out / k and v
+ * Bases are 16-byte aligned, strides multiples of 8. out overlaps no input. q_start, k_start: device int [nseq + 1]; q_rows / k_rows: rows that q and out / k and v
  * hold; max_q / max_k: the most rows of any one sequence (they size the launch). */
 typedef struct ork_b200_attn {
   const void *q, *k, *v;
@@ -219,8 +218,8 @@ int ork_b200_kv4_attn_async(ork_npu *ctx, const ork_b200_kv4 *c, const ork_b200_
 /* Eviction from a cache by accumulated attention weight. Of the n = len[s] tokens of each sequence and kv head,
  * min(n, keep) are kept: the first `sinks`, the last `recent`, then those with the largest score [nseq][Hkv][cap]
  * (ties: the lowest slot; a NaN counts as minus infinity); sinks + recent <= keep. The kept rows move, in their
- * order, from each of `nplanes` source planes src[i] [nseq][Hkv][cap] rows of row_bytes[i] (a multiple of 4, at most 65536) to
- * slots 0.. of dst[i] [nseq][Hkv][dcap], dcap >= keep: the planes of a 4-bit cache, or of an fp32 one. No source
+ * order, from each of `nplanes` source planes src[i] [nseq][Hkv][cap] rows of row_bytes[i] (a multiple of 4, at most
+ * 65536) to slots 0.. of dst[i] [nseq][Hkv][dcap], dcap >= keep: the planes of a 4-bit cache, or of an fp32 one. No source
  * overlaps a destination. kept [nseq][Hkv][keep]: the source slots (-1 past the kept ones); score_out
  * [nseq][Hkv][dcap]: their scores (0 up to `keep`), ready to accumulate on; len_out [nseq]: min(n, keep); it may be
  * len itself. kept, score_out and len_out may be NULL. max_len: the largest n. */
@@ -299,7 +298,7 @@ int ork_b200_device(const ork_npu *ctx);
  * weights while the previous kernel on the stream drains, and waits for that kernel before reading A. */
 int ork_b200_set_pdl(ork_npu *ctx, int on);
 /* Device bytes of run-time staging the context holds (host-buffer runs, grouped scales, decode-layer
- * workspace, ork_async pinned staging), all allocated on first use and grown on demand: 0 for a context
+ * workspace, ork_async pinned staging, the long-context workspace with what it keeps for captured graphs), all allocated on first use and grown on demand: 0 for a context
  * that has made no such call. For tests and tooling (e.g. that ork_i8_mm_run_noalloc allocated nothing). */
 size_t ork_b200_staging_bytes(const ork_npu *ctx);
 /* Number of kernels this context has launched (all kernels are this library's own). */

@@ -22,8 +22,8 @@
 //
 // Bound by the chain softmax -> P V -> Q K^T of each tile: a step of two tiles and 128 keys of 128 dims takes 3900
 // clocks, of which the tensor cores work 2050 to 2450 and the exponential unit 2050 (both 56 % active over the launch).
-// 16384 tokens, all visible, 16 heads of 128, bf16: 0.90 to 1.04 ms, 1.05 to 1.22 PFLOP/s; 8192 tokens of 64 heads, window
-// 1024: 390 us. Measured against: a step of 64 keys with two places for S, 1.58 ms; P handed over by halves, 1.02 ms;
+// 16384 tokens, all visible, 16 heads of 128, bf16: 0.86 to 1.04 ms, 1.05 to 1.27 PFLOP/s; 8192 tokens of 64 heads, window
+// 1024: 370 to 410 us. Measured against: a step of 64 keys with two places for S, 1.58 ms; P handed over by halves, 1.02 ms;
 // two threads a row, 0.93 to 1.02 ms.
 //
 // Every wait is bounded; one that expires records an error and the roles fall through to the common exit, which waits,

@@ -285,8 +285,9 @@ __global__ void __launch_bounds__(kRowThreads, STORE ? 4 : 1) kv4_rows_kernel(Ro
 // with 8 * sum(p * step) taken out again (the sum by a product with ones, so that it holds the rounded p * step), and
 // v is (c - 8) s + (b + 8 s).
 //
-// Bound by the instructions on the codes: 17.6 a token and kv head, issue slots 60 % and the tensor pipe 38 % used, at
-// 4.8 to 5.3 TB/s of cache (55 x 8 heads of 16384 bf16 tokens, 8 rows each: 197 us; the copies alone run at 6.4 TB/s).
+// Bound by the instructions on the codes: 17.9 a token and kv head, issue slots 60 % and the tensor pipe 37 % used, at
+// 5.0 to 5.3 TB/s of cache (55 x 8 heads of 16384 bf16 tokens, 8 rows each: 196 us; the copies alone run at 6.4 TB/s).
+// fp32 queries, 32 sequences of 8192 tokens, 64/8 heads of 128: 96 us.
 // Stages are requested by one elected lane at addresses that are the same in a warp by construction (uniform
 // registers): 13 % faster than a lane picked by its number.
 //
