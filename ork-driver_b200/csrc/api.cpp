@@ -13,6 +13,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <thread>
 #include <vector>
 
@@ -124,16 +125,21 @@ bool grow(void **p, size_t *cap, size_t need) {
 
 bool work_block(ork_npu *c, const char *name, Block *b, size_t need) {
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  const bool capturing = cudaStreamIsCapturing(c->stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone;
+  const bool unknown = cudaStreamIsCapturing(c->stream, &cs) != cudaSuccess, capturing = unknown || cs != cudaStreamCaptureStatusNone;
+  if (unknown) cudaGetLastError();
   if (b->cap < need) {
     if (capturing) {
-      cudaGetLastError();
       fprintf(stderr, "[ork] ERROR %s: the workspace would grow during CUDA-graph capture; make one call of this size "
                       "before capturing\n", name);
       return false;
     }
     if (b->graphed) {  // replays of the graph go on using it
-      c->outgrown.push_back(b->p);
+      try {
+        c->outgrown.push_back(b->p);
+      } catch (const std::bad_alloc &) {
+        fprintf(stderr, "[ork] ERROR %s: out of memory\n", name);
+        return false;
+      }
       c->capO += b->cap;
       *b = Block();
     }

@@ -1348,7 +1348,7 @@ int ork_b200_kv4_attn_async(ork_npu *c, const ork_b200_kv4 *kv, const ork_b200_k
     const long long span = a->window ? std::min<long long>(a->max_len, (long long)a->window + a->T + a->sinks + 3 * kUnit) : a->max_len;
     int unit = 1;  // tokens of whole column tiles
     while (unit < 2 * kRows && (a->H / kv->Hkv) * unit % (2 * kRows)) unit *= 2;
-    step = (int)std::min<long long>(step, std::max(kLogits / ((long long)kv->nseq * a->H * span * 4) / unit, 1ll) * unit);
+    step = (int)std::min<long long>(step, std::max(kLogits / 4 / span / ((long long)kv->nseq * a->H) / unit, 1ll) * unit);
   }
   Plan4 p = kv4_plan(kv, a, 0, step);
   size_t need = p.need, counts = p.counts;
