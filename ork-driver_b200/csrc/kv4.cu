@@ -278,12 +278,15 @@ __global__ void __launch_bounds__(kRowThreads, STORE ? 4 : 1) kv4_rows_kernel(Ro
 // So the row's largest p * step lies between 2^(kTop - 6) and 2^15 in one group at least. What is 2^-16 of it, and more,
 // is rounded to 11 bits (what is 2^-5 of it, and more, to 22), and smaller ones to 2^-27 of it: a token of large steps
 // that has no weight costs the others no digits, nor does a group of large steps the other group. With one scale of both
-// groups, by the largest step of the warp's tokens, a group of steps 10^4 times smaller was off by 6e-4 instead of 8e-7
-// (fp32 queries), and 32768 tokens 19 nats below another one by 7e-2 instead of 1e-6.
+// groups, by the largest step of the warp's tokens, a group of steps 10^4 times smaller was off by 6e-4 instead of 3e-7
+// (fp32 queries), and 32768 tokens 19 nats below another one by 7e-2 instead of 3e-6.
 // The codes of v are not negative although v has no sign: their sum would grow far above the output that it is to
 // leave after the lowest values' share is added, and the tensor cores truncate what they add. So each stage ends
 // with 8 * sum(p * step) taken out again (the sum by a product with ones, so that it holds the rounded p * step), and
-// v is (c - 8) s + (b + 8 s).
+// v is (c - 8) s + (b + 8 s). For fp32 queries the truncation shows all the same: it makes every unit's sum a little
+// smaller. There every other unit counts down, with -p * step and codes 15 - c, so that what one unit loses the next
+// brings back, and 7.5, the middle of the codes, is taken out: 131071 tokens came out off by 1.5e-6 to 2e-6 without,
+// 0.8e-6 to 1.1e-6 with it, 4000 tokens by 0.7e-6 and 0.5e-6. (16-bit queries would lose 5 % of their speed to it.)
 //
 // Bound by the instructions on the codes: 17.9 a token and kv head, issue slots 60 % and the tensor pipe 37 % used, at
 // 5.0 to 5.3 TB/s of cache (55 x 8 heads of 16384 bf16 tokens, 8 rows each: 196 us; the copies alone run at 6.4 TB/s).
@@ -430,7 +433,7 @@ struct Stage {  // one ring slot of a warp
   __half2 kp[kStageTok * (DK / kGroup)], vp[kStageTok * (DK / kGroup)];
 };
 // A stage's parameters in fp32: of each token the steps of its groups, then the lowest values (k), or the scaled steps
-// and b + 8 s (v).
+// and b + kMid s (v).
 template <int DK>
 struct Wide {
   float k[kStageTok][2 * (DK / kGroup)], v[kStageTok][2 * (DK / kGroup)];
@@ -500,6 +503,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
   constexpr int NG = DK / kGroup, NST = kStages<DK>, TR = NT * kRows;
   constexpr bool SPLIT = sizeof(E) == 4;
   constexpr int ND = kDigits<E>;
+  constexpr float kMid = SPLIT ? 7.5f : 8.0f;  // what the codes of v are taken from
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // known to be the same for the whole warp
@@ -616,6 +620,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
     }
   float vs[NG];  // scales of the groups' steps; 0 until a stage has any
   bool unset = true;
+  uint32_t flip = 0;  // all ones: units of even number count down (see above)
 #pragma unroll
   for (int g = 0; g < NG; g++) vs[g] = 0.0f;
   bool ok = true;
@@ -663,7 +668,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
 #pragma unroll
         for (int g = 0; g < NG; g++) {
           kpar[g] = kf[g].x, kpar[NG + g] = kf[g].y;
-          vpar[i][g] = vf[g].x, vpar[i][NG + g] = fmaf(8.0f, vf[g].x, vf[g].y);
+          vpar[i][g] = vf[g].x, vpar[i][NG + g] = fmaf(kMid, vf[g].x, vf[g].y);
         }
         store_pars(wide->k[tk], kpar);
       }
@@ -682,6 +687,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
           else unset = true;
         }
     }
+    const uint32_t down = SPLIT ? (flip ^ (lane & 16 ? ~0u : 0u)) & 0x80000000u : 0u;  // the sign of the lane's tokens' units
     float top[PT];  // the tokens' larger steps
 #pragma unroll
     for (int i = 0; i < PT; i++) {
@@ -689,7 +695,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
       top[i] = top[0];
       if (kStageTok % 32 == 0 || tk < kStageTok) {
 #pragma unroll
-        for (int g = 0; g < NG; g++) vpar[i][g] *= vs[g];
+        for (int g = 0; g < NG; g++) vpar[i][g] *= __uint_as_float(__float_as_uint(vs[g]) ^ down);
         store_pars(wide->v[tk], vpar[i]);
         top[i] = fmaxf(fabsf(vpar[i][0]), fabsf(vpar[i][NG - 1]));
       }
@@ -896,8 +902,9 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
           const uint32_t b0 = __byte_perm(wv[0], wv[1], sel), b1 = __byte_perm(wv[2], wv[3], sel);
           uint32_t af[4];
           if constexpr (SPLIT) {  // to bits 6 .. 9
-            af[0] = (j & 1 ? b0 >> 2 : b0 << 6) & 0x03c003c0u, af[1] = (j & 1 ? b0 >> 6 : b0 << 2) & 0x03c003c0u;
-            af[2] = (j & 1 ? b1 >> 2 : b1 << 6) & 0x03c003c0u, af[3] = (j & 1 ? b1 >> 6 : b1 << 2) & 0x03c003c0u;
+            const uint32_t f = w & 1 ? ~flip : flip;
+            af[0] = ((j & 1 ? b0 >> 2 : b0 << 6) ^ f) & 0x03c003c0u, af[1] = ((j & 1 ? b0 >> 6 : b0 << 2) ^ f) & 0x03c003c0u;
+            af[2] = ((j & 1 ? b1 >> 2 : b1 << 6) ^ f) & 0x03c003c0u, af[3] = ((j & 1 ? b1 >> 6 : b1 << 2) ^ f) & 0x03c003c0u;
           } else {
             const uint32_t s0 = j & 1 ? b0 >> 6 : b0 << 2, s1 = j & 1 ? b1 >> 6 : b1 << 2;
             af[0] = s0 & 0x003c003cu, af[1] = s0 & 0x03c003c0u, af[2] = s1 & 0x003c003cu, af[3] = s1 & 0x03c003c0u;
@@ -910,7 +917,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
         }
       }
     }
-    // take 8 * sum(p * step) out again, in the codes' units
+    // take kMid * sum(p * step) out again, in the codes' units
 #pragma unroll
     for (int y = 0; y < NT; y++)
 #pragma unroll
@@ -918,8 +925,9 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<E, DK, NT>) kv4_attn_kernel
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) o[y][g][j][i] = fmaf(sum[y][g][i & 1], SPLIT || i & 2 ? -0x1p-15f : -0x1p-19f, o[y][g][j][i]);
+          for (int i = 0; i < 4; i++) o[y][g][j][i] = fmaf(sum[y][g][i & 1], -kMid * (SPLIT || i & 2 ? 0x1p-18f : 0x1p-22f), o[y][g][j][i]);
     unit += cnt;
+    if constexpr (SPLIT) flip = ~flip;  // an odd number of units a stage
     __syncwarp();  // every lane has read the slot
     if (next < u1) {
       const int more = count(next);

@@ -419,3 +419,22 @@ def test_kv4_attn_weights_of_many_tokens_in_bounded_memory(on):
             c.put(s, rnd((n, 2, 64), 530 + s), rnd((n, 2, 64), 532 + s))
         attn4_check(own, c, rnd((2, T, 16, 64), 534, 1.5, torch.float16), lens, "f16")
         assert own.L.ork_b200_staging_bytes(own.ctx) < 6.5e9
+
+
+def test_kv4_attn_fp32_sums_over_a_long_context_have_no_drift(on):
+    # The logits' roundings, about 2^-20 of each weight, leave each output off by about 2^-20 A / sqrt(5000 tokens that
+    # count) = 1.4e-8 A, A = sum p |v|, to either side: 6e-10 A in the mean of 512 outputs. What the products truncate would
+    # all go one way; the mean may be off by 5e-9 A.
+    from test_gpu_longctx import Cache, attn4
+
+    n, H, Hkv, dk = 131000, 8, 2, 64
+    c = Cache(1, Hkv, dk, 131008)
+    bias = rnd((1, Hkv, dk), 540)
+    c.put(0, rnd((n, Hkv, dk), 541, 1.1) + bias, rnd((n, Hkv, dk), 542))
+    q = rnd((1, 1, H, dk), 543, 1.6)
+    rc, out = attn4(on, c, q, [n], "f32")
+    assert rc == 0 and on.L.ork_b200_sync(on.ctx) == 0
+    k, v = c.get(0, n)
+    want, size = ref.attention(q[0], k, v, dk ** -0.5, 0, 0)[0], ref.attention(q[0], k, v.abs(), dk ** -0.5, 0, 0)[0]
+    off = float((out[0].double() - want).mean() / size.mean())
+    assert abs(off) < 5e-9, off
